@@ -47,6 +47,7 @@ typedef struct CUstream_st* cudaStream_t;
 #define MUSA_KERNELS_EWORKSPACE (-2)  /* workspace missing or too small        */
 #define MUSA_KERNELS_EUNSUPPORTED (-3)/* dtype / activation code not known     */
 #define MUSA_KERNELS_ETOOLARGE (-4)   /* size beyond what the entry point holds */
+#define MUSA_KERNELS_EGAVEUP (-5)     /* a kernel's wait ran out (MusaMatMulStatus) */
 
 /* Library identity; lets a loader check that it found the sm_100a build. */
 const char* MusaKernelsVersion(void);
@@ -447,6 +448,101 @@ void LaunchRmsNormGradDxFloat(const float* x, const float* inv_rms, const float*
 void LaunchRmsNormGradDxBFloat16(const void* x, const void* inv_rms, const void* gamma,
                                  const void* dy, void* dx, int64_t num_rows,
                                  int64_t row_size, cudaStream_t stream);
+
+/* The residual's addition with the RMS norm behind it: sum = x + residual; inv_rms[row] =
+ * rsqrt(mean(sum^2) + epsilon), fp32; y = sum * inv_rms * gamma.  The norm is taken of the
+ * fp32 sum, `sum` holds it rounded to T.  x, residual, y, sum: [rows, row_size]. */
+int LaunchAddRmsNorm_F32(const void* x, const void* residual, const void* gamma, void* y,
+                         void* sum, float* inv_rms, int64_t rows, int64_t row_size,
+                         float epsilon, cudaStream_t stream);
+int LaunchAddRmsNorm_F16(const void* x, const void* residual, const void* gamma, void* y,
+                         void* sum, float* inv_rms, int64_t rows, int64_t row_size,
+                         float epsilon, cudaStream_t stream);
+int LaunchAddRmsNorm_BF16(const void* x, const void* residual, const void* gamma, void* y,
+                          void* sum, float* inv_rms, int64_t rows, int64_t row_size,
+                          float epsilon, cudaStream_t stream);
+
+/* Its gradient, from the stored sum and inv_rms: with g = dy * gamma and h = sum * inv_rms,
+ * dx = dsum + inv_rms * (g - h * mean_row(g * h)) (the gradient of x and of residual alike);
+ * dgamma = sum over rows of dy * h.  `dsum` (the gradient that reaches `sum` past the norm)
+ * may be null.  The column sums are added in a fixed order. */
+size_t AddRmsNormGradWorkspaceBytes(int64_t rows, int64_t row_size);
+int LaunchAddRmsNormGrad_F32(const void* dy, const void* dsum, const void* sum,
+                             const float* inv_rms, const void* gamma, void* dx, void* dgamma,
+                             int64_t rows, int64_t row_size, void* workspace,
+                             size_t workspace_bytes, cudaStream_t stream);
+int LaunchAddRmsNormGrad_F16(const void* dy, const void* dsum, const void* sum,
+                             const float* inv_rms, const void* gamma, void* dx, void* dgamma,
+                             int64_t rows, int64_t row_size, void* workspace,
+                             size_t workspace_bytes, cudaStream_t stream);
+int LaunchAddRmsNormGrad_BF16(const void* dy, const void* dsum, const void* sum,
+                              const float* inv_rms, const void* gamma, void* dx, void* dgamma,
+                              int64_t rows, int64_t row_size, void* workspace,
+                              size_t workspace_bytes, cudaStream_t stream);
+
+/* The same forward with its output in 8 bits: scale[row] = max(max|y| / 448, 2^-126), fp32;
+ * q = e4m3(y / scale), rounded to nearest even.  y is not written.  `residual` and `sum` may
+ * both be null (the norm of x alone); with `gamma` null too the rows of x are quantised as
+ * they are.  A NaN in a row makes its scale NaN. */
+int LaunchAddRmsNormQuantize_F32(const void* x, const void* residual, const void* gamma,
+                                 void* q, float* scale, void* sum, int64_t rows,
+                                 int64_t row_size, float epsilon, cudaStream_t stream);
+int LaunchAddRmsNormQuantize_F16(const void* x, const void* residual, const void* gamma,
+                                 void* q, float* scale, void* sum, int64_t rows,
+                                 int64_t row_size, float epsilon, cudaStream_t stream);
+int LaunchAddRmsNormQuantize_BF16(const void* x, const void* residual, const void* gamma,
+                                  void* q, float* scale, void* sum, int64_t rows,
+                                  int64_t row_size, float epsilon, cudaStream_t stream);
+
+/* ------------------------------------------------------- matrix products -- */
+
+/* z = op(a) op(b) + bias; y = act(z) + residual, one launch.  op(a) is [m, k]: memory holds
+ * it as lines of k elements `lda` apart, or (transpose_a) as lines of m elements; op(b) is
+ * [k, n]: lines of n, or (transpose_b) of k elements, `ldb` apart.  y, residual and
+ * preactivation (z rounded to T) are [m, n] without gaps; bias [n]; bias, residual and
+ * preactivation may be null.  dtype: MUSA_DT_F16 or MUSA_DT_BF16, of every tensor; products
+ * and epilogue are fp32, y is rounded once.  Tensor-core products: a factor that does not
+ * start on a 16-byte boundary, or whose lines are not a multiple of 16 bytes apart, is first
+ * copied to the workspace, whose size (0 where nothing is copied) the query gives.  The
+ * work of the reference's MusaLinearActivation and MusaMatMulBiasAdd
+ * (musa_ext/graph/fusion/linear_activation_fusion.cc:68-263). */
+#define MUSA_ACT_SILU 4     /* y = z * sigmoid(z): products only, see MUSA_ACT_SWISH */
+#define MUSA_ACT_GELU 5     /* y = z * Phi(z), Phi the normal distribution: products only */
+size_t MatMulWorkspaceBytes(int elem_bytes, const void* a, int64_t lda, bool transpose_a,
+                            const void* b, int64_t ldb, bool transpose_b, int64_t m, int64_t n,
+                            int64_t k);
+int LaunchMatMulBiasAct(int dtype, const void* a, int64_t lda, bool transpose_a, const void* b,
+                        int64_t ldb, bool transpose_b, const void* bias, const void* residual,
+                        void* y, void* preactivation, int64_t m, int64_t n, int64_t k, int act,
+                        void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/* Its gradient: dz = dy * act'(preactivation); da and db (without gaps, laid out as a and b:
+ * [k, m] / [n, k] where transposed) are the products of dz, rounded to T, with the other
+ * factor; dbias the column sums of the unrounded dz, added in a fixed order.  The gradient
+ * of the residual is dy.  da, db and dbias may be null; preactivation is not read with
+ * MUSA_ACT_IDENTITY. */
+size_t MatMulGradWorkspaceBytes(const void* dy, const void* a, int64_t lda, bool transpose_a,
+                                const void* b, int64_t ldb, bool transpose_b, int64_t m,
+                                int64_t n, int64_t k, int act);
+int LaunchMatMulBiasActGrad(int dtype, const void* dy, const void* a, int64_t lda,
+                            bool transpose_a, const void* b, int64_t ldb, bool transpose_b,
+                            const void* preactivation, void* da, void* db, void* dbias,
+                            int64_t m, int64_t n, int64_t k, int act, void* workspace,
+                            size_t workspace_bytes, cudaStream_t stream);
+
+/* The product of e4m3 factors with fp32 scales: z = (a b^T) * a_scale[row] * b_scale[column]
+ * + bias; y = act(z) + residual.  a: lines of k bytes, `lda` apart, [m, k]; b: [n, k].  bias,
+ * residual and y are of out_dtype (MUSA_DT_F16 or MUSA_DT_BF16). */
+int LaunchQuantizedMatMulBiasAct(int out_dtype, const void* a, int64_t lda,
+                                 const float* a_scale, const void* b, int64_t ldb,
+                                 const float* b_scale, const void* bias, const void* residual,
+                                 void* y, int64_t m, int64_t n, int64_t k, int act,
+                                 void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/* MUSA_KERNELS_OK, or MUSA_KERNELS_EGAVEUP once a product's kernel on the current device
+ * has given up a wait (its outputs are then not valid); the waits end after about two
+ * seconds, which no launch comes near.  Synchronises with the device. */
+int MusaMatMulStatus(void);
 
 /* ------------------------------------------------------ FusedBatchNorm -- */
 

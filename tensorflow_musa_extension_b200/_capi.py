@@ -145,6 +145,29 @@ PROTOTYPES = {
          + [c_i64, c_i64, c_i64, c_f32, c_vp]),
 }
 
+_ADD_RMS_NORM = [c_vp] * 6 + [c_i64, c_i64, c_f32, c_vp]
+_ADD_RMS_NORM_GRAD = [c_vp] * 7 + [c_i64, c_i64, c_vp, c_size, c_vp]
+_FACTORS = [c_vp, c_i64, c_bool, c_vp, c_i64, c_bool]
+
+PROTOTYPES.update({
+    "AddRmsNormGradWorkspaceBytes": (c_size, [c_i64, c_i64]),
+    "MatMulWorkspaceBytes": (c_size, [c_int] + _FACTORS + [c_i64] * 3),
+    "LaunchMatMulBiasAct":
+        (c_int, [c_int] + _FACTORS + [c_vp] * 4 + [c_i64] * 3 + [c_int, c_vp, c_size, c_vp]),
+    "MatMulGradWorkspaceBytes": (c_size, [c_vp] + _FACTORS + [c_i64] * 3 + [c_int]),
+    "LaunchMatMulBiasActGrad":
+        (c_int, [c_int, c_vp] + _FACTORS + [c_vp] * 4 + [c_i64] * 3
+         + [c_int, c_vp, c_size, c_vp]),
+    "LaunchQuantizedMatMulBiasAct":
+        (c_int, [c_int, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp] + [c_vp] * 3 + [c_i64] * 3
+         + [c_int, c_vp, c_size, c_vp]),
+    "MusaMatMulStatus": (c_int, []),
+})
+for _suffix in ("F32", "F16", "BF16"):
+    PROTOTYPES["LaunchAddRmsNorm_" + _suffix] = (c_int, _ADD_RMS_NORM)
+    PROTOTYPES["LaunchAddRmsNormGrad_" + _suffix] = (c_int, _ADD_RMS_NORM_GRAD)
+    PROTOTYPES["LaunchAddRmsNormQuantize_" + _suffix] = (c_int, _ADD_RMS_NORM)
+
 PROTOTYPES.update({
     "MusaExchangeCreate": (c_vp, [c_int, c_int, c_i64]),
     "MusaExchangeIpcHandle": (c_int, [c_vp, c_vp]),
@@ -235,6 +258,7 @@ ERROR_NAMES = {
     -2: "workspace missing, misaligned or too small",
     -3: "unsupported dtype or activation code",
     -4: "size beyond what the entry point holds",
+    -5: "a kernel gave up a wait: its outputs are not valid",
 }
 
 

@@ -1,0 +1,616 @@
+// The residual's addition with the RMS norm behind it, its gradient, and the same
+// forward with an 8-bit output.
+//
+//   s = x + residual;  inv = rsqrt(mean(s^2) + eps);  y = s * inv * gamma
+//   scale = max(max|y| / 448, 2^-126);  q = e4m3(y / scale)
+//   g = dy * gamma;  h = s * inv;  dx = dsum + inv * (g - h * mean(g * h))
+//   dgamma = sum over rows of dy * h
+//
+// Bound by memory: 4 * sizeof(T) per element forward (x, residual in; y, sum out) and
+// backward (dy, dsum, sum in; dx out), 3 * sizeof(T) + 1 with the 8-bit output.  A row is
+// read once: a group of threads holds it in registers as fp32 sums.  The row's sum of
+// squares and largest |s * gamma| come from one round of reductions, the 8-bit scale from
+// both, so the 16-bit y is never written.
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "partial_rows.cuh"
+#include "row_layout.h"
+#include "trace.h"
+#include "../../include/musa_plugin_kernels.h"
+
+namespace musa_b200 {
+namespace {
+
+constexpr float kE4m3Max = 448.0f;
+constexpr float kScaleMin = 1.17549435e-38f;  // 2^-126
+
+struct AddNormArgs {
+  const void* x;
+  const void* residual;  // may be null with the 8-bit output
+  const void* gamma;     // may be null with the 8-bit output (rows as they are)
+  void* y;               // y of type T, or q
+  void* sum;
+  float* stat;           // inv_rms, or scale
+  int64_t rows;
+  int row_size;
+  int group;             // threads of a row, a power of two
+  float epsilon;
+};
+
+// Sum of `v` and largest of `w` over the group's threads (power of two, aligned runs).
+__device__ __forceinline__ void GroupSumMax(float& v, unsigned& w, int group, float* sums,
+                                            unsigned* tops) {
+  const int span = group < 32 ? group : 32;
+  for (int m = span / 2; m > 0; m >>= 1) {
+    v += __shfl_xor_sync(0xffffffffu, v, m);
+    w = max(w, __shfl_xor_sync(0xffffffffu, w, m));
+  }
+  if (group > 32) {
+    const int warp = threadIdx.x >> 5, warps = group >> 5;
+    const int first = warp & ~(warps - 1);
+    if ((threadIdx.x & 31) == 0) {
+      sums[warp] = v;
+      tops[warp] = w;
+    }
+    __syncthreads();
+    v = 0.0f;
+    w = 0;
+    for (int i = 0; i < warps; ++i) {
+      v += sums[first + i];
+      w = max(w, tops[first + i]);
+    }
+  }
+}
+
+// |v| as bits that order like the values, NaN above all.
+__device__ __forceinline__ unsigned MagnitudeBits(float v) {
+  return __float_as_uint(v) & 0x7fffffffu;
+}
+
+__device__ __forceinline__ float QuantizeScale(float top) {
+  const float t = top / kE4m3Max;
+  return t < kScaleMin ? kScaleMin : t;  // NaN goes through
+}
+
+// y / scale.  Rows quantised as they are take the rounded division: quotients of 16-bit
+// values fall on borders between two e4m3 values, where a last bit decides.  Behind a norm
+// the fp32 values are off by more than the product with the reciprocal.
+__device__ __forceinline__ float Quotient(float y, float scale, float unscale, bool normed) {
+  return normed ? y * unscale : y / scale;
+}
+
+template <int kVec>
+__device__ __forceinline__ Pack<uint8_t, kVec> ToE4m3(const float (&v)[kVec]) {
+  Pack<uint8_t, kVec> out;
+  uint16_t* w = reinterpret_cast<uint16_t*>(&out);
+#pragma unroll
+  for (int i = 0; i < kVec / 2; ++i) {
+    w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE,
+                                    __NV_E4M3);
+  }
+  return out;
+}
+
+// A row's packs against the tensor: whole packs, or (kShifted) rows of any length, whose
+// first and last pack may hold elements of the neighbouring rows.
+template <typename T, bool kShifted>
+struct RowView {
+  static constexpr int kVec = VecWidth<T>::value;
+  int64_t first;  // element of the row's first pack
+  int64_t total;  // elements of the tensor
+  int shift, packs, row_size;
+  __device__ RowView(int64_t row, int64_t rows, int size) : row_size(size) {
+    total = rows * size;
+    if constexpr (kShifted) {
+      shift = RowShift<kVec>(row, size);
+      packs = ShiftedPacks<kVec>(size, shift);
+      first = row * size - shift;
+    } else {
+      shift = 0;
+      packs = size / kVec;
+      first = row * size;
+    }
+  }
+  __device__ bool Edge(int p) const { return kShifted && (p == 0 || p == packs - 1); }
+  __device__ bool Inside(int p, int e) const {
+    return static_cast<unsigned>(p * kVec + e - shift) < static_cast<unsigned>(row_size);
+  }
+  __device__ Pack<T, kVec> Load(const void* base, int p) const {
+    const T* at = static_cast<const T*>(base) + first + p * kVec;
+    if (kShifted && first + (p + 1) * static_cast<int64_t>(kVec) > total) {
+      Pack<T, kVec> v;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v.v[e] = Inside(p, e) ? at[e] : FromF32<T>(0.0f);
+      return v;
+    }
+    return LoadStream(reinterpret_cast<const Pack<T, kVec>*>(at));
+  }
+  template <typename U>
+  __device__ void Store(void* base, int p, const Pack<U, kVec>& v) const {
+    U* at = static_cast<U*>(base) + first + p * kVec;
+    if (Edge(p)) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        if (Inside(p, e)) at[e] = v.v[e];
+      }
+    } else {
+      StoreStream(reinterpret_cast<Pack<U, kVec>*>(at), v);
+    }
+  }
+  // A vector of row_size values (gamma) where pack p's elements are.
+  __device__ Pack<T, kVec> Vector(const void* base, int p) const {
+    const T* at = static_cast<const T*>(base) + p * kVec - shift;
+    if constexpr (kShifted) {
+      Pack<T, kVec> v;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v.v[e] = Inside(p, e) ? at[e] : FromF32<T>(0.0f);
+      return v;
+    } else {
+      return LoadKeep(reinterpret_cast<const Pack<T, kVec>*>(at));
+    }
+  }
+};
+
+template <typename T, int kPacks, bool kQuantize, bool kShifted>
+__global__ void __launch_bounds__(1024) AddNormKernel(AddNormArgs a) {
+  constexpr int kVec = VecWidth<T>::value;
+  using P = Pack<T, kVec>;
+  __shared__ float sums[32];
+  __shared__ unsigned tops[32];
+  const int t = threadIdx.x & (a.group - 1);
+  const int64_t row =
+      static_cast<int64_t>(blockIdx.x) * (blockDim.x / a.group) + threadIdx.x / a.group;
+  const bool there = row < a.rows;
+  const RowView<T, kShifted> view(there ? row : 0, a.rows, a.row_size);
+  P x[kPacks], r[kPacks], gamma[kPacks];
+  float s[kPacks][kVec];
+#pragma unroll
+  for (int j = 0; j < kPacks; ++j) {
+    const int p = t + j * a.group;
+    if (there && p < view.packs) {
+      x[j] = view.Load(a.x, p);
+      if (!kQuantize || a.residual != nullptr) r[j] = view.Load(a.residual, p);
+      if (!kQuantize || a.gamma != nullptr) gamma[j] = view.Vector(a.gamma, p);
+    }
+  }
+  float square = 0.0f;
+  unsigned top = 0;
+#pragma unroll
+  for (int j = 0; j < kPacks; ++j) {
+    const int p = t + j * a.group;
+    if (there && p < view.packs) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        s[j][e] = ToF32(x[j].v[e]);
+        if (!kQuantize || a.residual != nullptr) s[j][e] += ToF32(r[j].v[e]);
+        if (view.Edge(p) && !view.Inside(p, e)) s[j][e] = 0.0f;
+        square = fmaf(s[j][e], s[j][e], square);
+        if constexpr (kQuantize) {
+          const float g = a.gamma != nullptr ? ToF32(gamma[j].v[e]) : 1.0f;
+          top = max(top, MagnitudeBits(s[j][e] * g));
+        }
+      }
+    }
+  }
+  GroupSumMax(square, top, a.group, sums, tops);
+  float inv = rsqrtf(square / a.row_size + a.epsilon);
+  if (kQuantize && a.gamma == nullptr) inv = 1.0f;
+  float scale = 1.0f, unscale = 1.0f;
+  if constexpr (kQuantize) {
+    scale = QuantizeScale(__uint_as_float(top) * inv);
+    unscale = 1.0f / scale;
+    if (there && t == 0) a.stat[row] = scale;
+  } else {
+    if (there && t == 0) a.stat[row] = inv;
+  }
+#pragma unroll
+  for (int j = 0; j < kPacks; ++j) {
+    const int p = t + j * a.group;
+    if (there && p < view.packs) {
+      P total;
+      float y[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        total.v[e] = FromF32<T>(s[j][e]);
+        const float g = !kQuantize || a.gamma != nullptr ? ToF32(gamma[j].v[e]) : 1.0f;
+        y[e] = s[j][e] * inv * g;
+      }
+      if (!kQuantize || a.sum != nullptr) view.Store(a.sum, p, total);
+      if constexpr (kQuantize) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) y[e] = Quotient(y[e], scale, unscale, a.gamma != nullptr);
+        view.Store(a.y, p, ToE4m3<kVec>(y));
+      } else {
+        P out;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) out.v[e] = FromF32<T>(y[e]);
+        view.Store(a.y, p, out);
+      }
+    }
+  }
+}
+
+// Rows of any length and alignment: a CTA walks its row twice, element by element.
+constexpr int kLoopThreads = 512;
+
+template <typename T, bool kQuantize>
+__global__ void __launch_bounds__(kLoopThreads) AddNormLoopKernel(AddNormArgs a) {
+  __shared__ float sums[32];
+  __shared__ unsigned tops[32];
+  const T* gamma = static_cast<const T*>(a.gamma);
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + row * a.row_size;
+    const T* r = a.residual != nullptr ? static_cast<const T*>(a.residual) + row * a.row_size
+                                       : nullptr;
+    const auto Sum = [&](int c) { return r != nullptr ? ToF32(x[c]) + ToF32(r[c]) : ToF32(x[c]); };
+    float square = 0.0f;
+    unsigned top = 0;
+    for (int c = threadIdx.x; c < a.row_size; c += kLoopThreads) {
+      const float s = Sum(c);
+      square = fmaf(s, s, square);
+      if (kQuantize) top = max(top, MagnitudeBits(gamma != nullptr ? s * ToF32(gamma[c]) : s));
+    }
+    GroupSumMax(square, top, kLoopThreads, sums, tops);
+    __syncthreads();  // before the next row's sums
+    float inv = rsqrtf(square / a.row_size + a.epsilon);
+    if (kQuantize && gamma == nullptr) inv = 1.0f;
+    const float scale = kQuantize ? QuantizeScale(__uint_as_float(top) * inv) : 1.0f;
+    const float unscale = 1.0f / scale;
+    if (threadIdx.x == 0) a.stat[row] = kQuantize ? scale : inv;
+    for (int c = threadIdx.x; c < a.row_size; c += kLoopThreads) {
+      const float s = Sum(c);
+      const int64_t at = row * a.row_size + c;
+      if (a.sum != nullptr) static_cast<T*>(a.sum)[at] = FromF32<T>(s);
+      const float y = s * inv * (gamma != nullptr ? ToF32(gamma[c]) : 1.0f);
+      if constexpr (kQuantize) {
+        static_cast<uint8_t*>(a.y)[at] =
+            __nv_cvt_float_to_fp8(Quotient(y, scale, unscale, gamma != nullptr), __NV_SATFINITE,
+                                  __NV_E4M3);
+      } else {
+        static_cast<T*>(a.y)[at] = FromF32<T>(y);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- gradient --
+
+struct AddNormGradArgs {
+  const void* dy;
+  const void* dsum;   // may be null
+  const void* sum;
+  const float* inv;
+  const void* gamma;
+  void* dx;
+  float* partial;     // [gridDim.x][row_size]
+  int64_t rows;
+  int row_size;
+  int group;
+};
+
+// A thread meets the same columns in each of its rows (shifted rows: they are a multiple
+// of the pack width apart, the launch sees to it) and keeps their dgamma in registers.  At
+// the end the row lanes of the CTA are added in order and the CTA leaves one partial row.
+constexpr int kGradThreads = 512;
+
+template <typename T, int kPacks, bool kShifted>
+__global__ void __launch_bounds__(kGradThreads) AddNormGradKernel(AddNormGradArgs a) {
+  constexpr int kVec = VecWidth<T>::value;
+  using P = Pack<T, kVec>;
+  __shared__ float sums[2][32];
+  __shared__ unsigned tops[2][32];
+  extern __shared__ float columns[];
+  const int t = threadIdx.x & (a.group - 1);
+  const int lane_row = threadIdx.x / a.group, lanes = blockDim.x / a.group;
+  float acc[kPacks][kVec];
+#pragma unroll
+  for (int j = 0; j < kPacks; ++j) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) acc[j][e] = 0.0f;
+  }
+  const int64_t first_row = static_cast<int64_t>(blockIdx.x) * lanes + lane_row;
+  int parity = 0;
+  // Whole CTAs go round: the reductions of wide groups are barriers.
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * lanes; base < a.rows;
+       base += static_cast<int64_t>(gridDim.x) * lanes) {
+    const int64_t row = base + lane_row;
+    const bool there = row < a.rows;
+    const RowView<T, kShifted> view(there ? row : 0, a.rows, a.row_size);
+    P s[kPacks], dy[kPacks], ds[kPacks];
+    float inv = 0.0f;
+    if (there) {
+      inv = a.inv[row];
+#pragma unroll
+      for (int j = 0; j < kPacks; ++j) {
+        const int p = t + j * a.group;
+        if (p < view.packs) {
+          s[j] = view.Load(a.sum, p);
+          dy[j] = view.Load(a.dy, p);
+          if (a.dsum != nullptr) ds[j] = view.Load(a.dsum, p);
+        }
+      }
+    }
+    float dot = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPacks; ++j) {
+      const int p = t + j * a.group;
+      if (there && p < view.packs) {
+        const P gamma = view.Vector(a.gamma, p);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          if (view.Edge(p) && !view.Inside(p, e)) {
+            s[j].v[e] = FromF32<T>(0.0f);
+            dy[j].v[e] = FromF32<T>(0.0f);
+          }
+          const float dh = ToF32(dy[j].v[e]) * (ToF32(s[j].v[e]) * inv);
+          acc[j][e] += dh;
+          dot = fmaf(dh, ToF32(gamma.v[e]), dot);
+        }
+      }
+    }
+    unsigned none = 0;
+    GroupSumMax(dot, none, a.group, sums[parity], tops[parity]);
+    parity ^= 1;
+    const float mean = dot / a.row_size;
+#pragma unroll
+    for (int j = 0; j < kPacks; ++j) {
+      const int p = t + j * a.group;
+      if (there && p < view.packs) {
+        const P gamma = view.Vector(a.gamma, p);
+        P out;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          const float g = ToF32(dy[j].v[e]) * ToF32(gamma.v[e]);
+          float d = inv * (g - ToF32(s[j].v[e]) * inv * mean);
+          if (a.dsum != nullptr) d += ToF32(ds[j].v[e]);
+          out.v[e] = FromF32<T>(d);
+        }
+        view.Store(a.dx, p, out);
+      }
+    }
+  }
+  float* partial = a.partial + static_cast<int64_t>(blockIdx.x) * a.row_size;
+  const RowView<T, kShifted> view(first_row, a.rows, a.row_size);
+  if (lanes == 1) {
+#pragma unroll
+    for (int j = 0; j < kPacks; ++j) {
+      const int p = t + j * a.group;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        if (p < view.packs && view.Inside(p, e)) partial[p * kVec + e - view.shift] = acc[j][e];
+      }
+    }
+    return;
+  }
+  for (int c = threadIdx.x; c < a.row_size; c += blockDim.x) columns[c] = 0.0f;
+  __syncthreads();
+  for (int l = 0; l < lanes; ++l) {
+    if (l == lane_row && first_row < a.rows) {
+#pragma unroll
+      for (int j = 0; j < kPacks; ++j) {
+        const int p = t + j * a.group;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          if (p < view.packs && view.Inside(p, e)) columns[p * kVec + e - view.shift] += acc[j][e];
+        }
+      }
+    }
+    __syncthreads();
+  }
+  for (int c = threadIdx.x; c < a.row_size; c += blockDim.x) partial[c] = columns[c];
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLoopThreads) AddNormGradLoopKernel(AddNormGradArgs a) {
+  __shared__ float sums[2][32];
+  __shared__ unsigned tops[2][32];
+  const T* gamma = static_cast<const T*>(a.gamma);
+  float* partial = a.partial + static_cast<int64_t>(blockIdx.x) * a.row_size;
+  for (int c = threadIdx.x; c < a.row_size; c += kLoopThreads) partial[c] = 0.0f;
+  int parity = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* s = static_cast<const T*>(a.sum) + row * a.row_size;
+    const T* dy = static_cast<const T*>(a.dy) + row * a.row_size;
+    const float inv = a.inv[row];
+    float dot = 0.0f;
+    for (int c = threadIdx.x; c < a.row_size; c += kLoopThreads) {
+      const float dh = ToF32(dy[c]) * (ToF32(s[c]) * inv);
+      partial[c] += dh;
+      dot = fmaf(dh, ToF32(gamma[c]), dot);
+    }
+    unsigned none = 0;
+    GroupSumMax(dot, none, kLoopThreads, sums[parity], tops[parity]);
+    parity ^= 1;
+    const float mean = dot / a.row_size;
+    for (int c = threadIdx.x; c < a.row_size; c += kLoopThreads) {
+      const int64_t at = row * a.row_size + c;
+      float d = inv * (ToF32(dy[c]) * ToF32(gamma[c]) - ToF32(s[c]) * inv * mean);
+      if (a.dsum != nullptr) d += ToF32(static_cast<const T*>(a.dsum)[at]);
+      static_cast<T*>(a.dx)[at] = FromF32<T>(d);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- launches --
+
+inline bool BadRows(int64_t rows, int64_t row_size) {
+  return rows < 0 || row_size < 0 || row_size > (int64_t(1) << 24);
+}
+
+int PowerOfTwoAtLeast(int64_t v, int low) {
+  int p = low;
+  while (p < v) p *= 2;
+  return p;
+}
+
+template <typename T, bool kQuantize>
+int LaunchForward(AddNormArgs a, bool aligned, cudaStream_t stream) {
+  constexpr int kVec = VecWidth<T>::value;
+  const bool shifted = a.row_size % kVec != 0;
+  const int64_t packs = CeilDiv(a.row_size, kVec) + (shifted ? 1 : 0);
+  CountKernelLaunch();
+  if (!aligned || packs > 4 * 1024) {
+    const int64_t ctas = a.rows < SmCount() * 4 ? a.rows : SmCount() * 4;
+    AddNormLoopKernel<T, kQuantize><<<static_cast<unsigned>(ctas), kLoopThreads, 0, stream>>>(a);
+    return static_cast<int>(cudaGetLastError());
+  }
+  // Two packs a thread; one where rows are few (a call is all latency), four where a row
+  // needs them.
+  int per_thread = a.rows <= SmCount() ? 1 : 2;
+  if (packs > per_thread * 1024) per_thread = packs > 2048 ? 4 : 2;
+  a.group = PowerOfTwoAtLeast(CeilDiv(packs, per_thread), 8);
+  const int threads = a.group > 256 ? a.group : 256;
+  const dim3 grid(static_cast<unsigned>(CeilDiv(a.rows, threads / a.group)));
+#define MUSA_RUN(PACKS)                                                        \
+  (shifted ? AddNormKernel<T, PACKS, kQuantize, true><<<grid, threads, 0, stream>>>(a) \
+           : AddNormKernel<T, PACKS, kQuantize, false><<<grid, threads, 0, stream>>>(a))
+  if (per_thread == 1) MUSA_RUN(1);
+  else if (per_thread == 2) MUSA_RUN(2);
+  else MUSA_RUN(4);
+#undef MUSA_RUN
+  return static_cast<int>(cudaGetLastError());
+}
+
+// The most CTAs of a gradient, a multiple of eight: their partial rows stay below 64 MB (or
+// at eight rows).
+int MostGradCtas(int64_t row_size) {
+  const int64_t by_size = (int64_t(16) << 20) / row_size;
+  const int64_t most = by_size < SmCount() * 4 ? by_size : SmCount() * 4;
+  return most < 8 ? 8 : static_cast<int>(most / 8 * 8);
+}
+
+template <typename T>
+int LaunchGrad(AddNormGradArgs a, bool aligned, void* dgamma, cudaStream_t stream) {
+  constexpr int kVec = VecWidth<T>::value;
+  const bool shifted = a.row_size % kVec != 0;
+  const int64_t packs = CeilDiv(a.row_size, kVec) + (shifted ? 1 : 0);
+  const int most = MostGradCtas(a.row_size);
+  int ctas;
+  CountKernelLaunch();
+  if (!aligned || packs > 4 * kGradThreads) {
+    ctas = static_cast<int>(a.rows < most ? a.rows : most);
+    AddNormGradLoopKernel<T><<<ctas, kLoopThreads, 0, stream>>>(a);
+  } else {
+    const int per_thread = packs > 2 * kGradThreads ? 4 : 2;
+    a.group = PowerOfTwoAtLeast(CeilDiv(packs, per_thread), 8);
+    const int threads = a.group > 256 ? a.group : 256;
+    const int lanes = threads / a.group;
+    int64_t want = CeilDiv(a.rows, lanes);
+    if (want > most) want = most;
+    // Shifted rows: a thread's rows are a multiple of the pack width apart.
+    if (shifted && want * lanes < a.rows) want = want / kVec * kVec;
+    ctas = static_cast<int>(want);
+    const size_t smem = lanes > 1 ? sizeof(float) * a.row_size : 0;
+#define MUSA_RUN(PACKS)                                                              \
+  (shifted ? AddNormGradKernel<T, PACKS, true><<<ctas, threads, smem, stream>>>(a)   \
+           : AddNormGradKernel<T, PACKS, false><<<ctas, threads, smem, stream>>>(a))
+    if (per_thread == 2) MUSA_RUN(2);
+    else MUSA_RUN(4);
+#undef MUSA_RUN
+  }
+  const cudaError_t rc = cudaGetLastError();
+  if (rc != cudaSuccess) return static_cast<int>(rc);
+  return static_cast<int>(
+      LaunchAddPartialRows<T>(false, a.partial, ctas, a.row_size, dgamma, stream));
+}
+
+template <typename T>
+int AddNorm(const void* x, const void* residual, const void* gamma, void* y, void* sum,
+            float* inv_rms, int64_t rows, int64_t row_size, float epsilon, cudaStream_t stream) {
+  if (BadRows(rows, row_size)) return MUSA_KERNELS_EINVAL;
+  MUSA_TRACE("LaunchAddRmsNorm", 4 * sizeof(T) * rows * row_size);
+  if (rows == 0 || row_size == 0) return MUSA_KERNELS_OK;
+  if (x == nullptr || residual == nullptr || gamma == nullptr || y == nullptr || sum == nullptr ||
+      inv_rms == nullptr) {
+    return MUSA_KERNELS_EINVAL;
+  }
+  const bool aligned = Aligned16(x) && Aligned16(residual) && Aligned16(gamma) && Aligned16(y) &&
+                       Aligned16(sum);
+  return LaunchForward<T, false>({x, residual, gamma, y, sum, inv_rms, rows,
+                                  static_cast<int>(row_size), 0, epsilon},
+                                 aligned, stream);
+}
+
+template <typename T>
+int AddNormQuantize(const void* x, const void* residual, const void* gamma, void* q, float* scale,
+                    void* sum, int64_t rows, int64_t row_size, float epsilon,
+                    cudaStream_t stream) {
+  if (BadRows(rows, row_size)) return MUSA_KERNELS_EINVAL;
+  MUSA_TRACE("LaunchAddRmsNormQuantize",
+             ((residual != nullptr ? 3 : 1) * sizeof(T) + 1) * rows * row_size);
+  if (rows == 0 || row_size == 0) return MUSA_KERNELS_OK;
+  if (x == nullptr || q == nullptr || scale == nullptr ||
+      (residual == nullptr) != (sum == nullptr) || (residual != nullptr && gamma == nullptr)) {
+    return MUSA_KERNELS_EINVAL;
+  }
+  const bool aligned = Aligned16(x) && Aligned16(residual) && Aligned16(gamma) && Aligned16(q) &&
+                       Aligned16(sum);
+  return LaunchForward<T, true>({x, residual, gamma, q, sum, scale, rows,
+                                 static_cast<int>(row_size), 0, epsilon},
+                                aligned, stream);
+}
+
+template <typename T>
+int AddNormGrad(const void* dy, const void* dsum, const void* sum, const float* inv_rms,
+                const void* gamma, void* dx, void* dgamma, int64_t rows, int64_t row_size,
+                void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  if (BadRows(rows, row_size)) return MUSA_KERNELS_EINVAL;
+  MUSA_TRACE("LaunchAddRmsNormGrad",
+             (dsum != nullptr ? 4 : 3) * sizeof(T) * rows * row_size);
+  if (row_size == 0) return MUSA_KERNELS_OK;
+  if (dgamma == nullptr) return MUSA_KERNELS_EINVAL;
+  if (rows == 0) return static_cast<int>(cudaMemsetAsync(dgamma, 0, sizeof(T) * row_size, stream));
+  if (dy == nullptr || sum == nullptr || inv_rms == nullptr || gamma == nullptr ||
+      dx == nullptr) {
+    return MUSA_KERNELS_EINVAL;
+  }
+  const size_t need = static_cast<size_t>(MostGradCtas(row_size)) * row_size * sizeof(float);
+  if (workspace == nullptr || workspace_bytes < need || !Aligned16(workspace)) {
+    return MUSA_KERNELS_EWORKSPACE;
+  }
+  const bool aligned = Aligned16(dy) && Aligned16(dsum) && Aligned16(sum) && Aligned16(gamma) &&
+                       Aligned16(dx);
+  return LaunchGrad<T>({dy, dsum, sum, inv_rms, gamma, dx, static_cast<float*>(workspace), rows,
+                        static_cast<int>(row_size), 0},
+                       aligned, dgamma, stream);
+}
+
+}  // namespace
+}  // namespace musa_b200
+
+using namespace musa_b200;
+
+extern "C" {
+
+size_t AddRmsNormGradWorkspaceBytes(int64_t rows, int64_t row_size) {
+  if (BadRows(rows, row_size) || rows == 0 || row_size == 0) return 0;
+  return static_cast<size_t>(MostGradCtas(row_size)) * row_size * sizeof(float);
+}
+
+#define MUSA_DEFINE_ADD_RMS_NORM(SUFFIX, TYPE)                                                   \
+  int LaunchAddRmsNorm_##SUFFIX(const void* x, const void* residual, const void* gamma, void* y, \
+                                void* sum, float* inv_rms, int64_t rows, int64_t row_size,       \
+                                float epsilon, cudaStream_t stream) {                            \
+    return AddNorm<TYPE>(x, residual, gamma, y, sum, inv_rms, rows, row_size, epsilon, stream);  \
+  }                                                                                              \
+  int LaunchAddRmsNormGrad_##SUFFIX(const void* dy, const void* dsum, const void* sum,           \
+                                    const float* inv_rms, const void* gamma, void* dx,           \
+                                    void* dgamma, int64_t rows, int64_t row_size,                \
+                                    void* workspace, size_t workspace_bytes,                     \
+                                    cudaStream_t stream) {                                       \
+    return AddNormGrad<TYPE>(dy, dsum, sum, inv_rms, gamma, dx, dgamma, rows, row_size,          \
+                             workspace, workspace_bytes, stream);                                \
+  }                                                                                              \
+  int LaunchAddRmsNormQuantize_##SUFFIX(const void* x, const void* residual, const void* gamma,  \
+                                        void* q, float* scale, void* sum, int64_t rows,          \
+                                        int64_t row_size, float epsilon, cudaStream_t stream) {  \
+    return AddNormQuantize<TYPE>(x, residual, gamma, q, scale, sum, rows, row_size, epsilon,     \
+                                 stream);                                                        \
+  }
+MUSA_DEFINE_ADD_RMS_NORM(F32, float)
+MUSA_DEFINE_ADD_RMS_NORM(F16, __half)
+MUSA_DEFINE_ADD_RMS_NORM(BF16, __nv_bfloat16)
+#undef MUSA_DEFINE_ADD_RMS_NORM
+
+}  // extern "C"

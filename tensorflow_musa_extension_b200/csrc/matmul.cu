@@ -1,0 +1,778 @@
+// Matrix products with bias, activation and residual in the epilogue, and their gradient.
+//
+//   z = op(a) op(b) + bias          op(a) [m, k], op(b) [k, n]
+//   y = act(z) + residual           act in {identity, relu, sigmoid, silu, gelu}
+//
+// 16-bit factors (half, bfloat16), or e4m3 factors with one fp32 scale per row of a and
+// per column of the product.  The products run on the tensor cores (tcgen05, fp32
+// accumulators in tensor memory), fed by TMA through a ring of shared-memory stages;
+// everything after the product is fp32 arithmetic on the accumulators, rounded once.
+// A factor stored transposed is read as it lies: the matrix instructions take both
+// orders.  A factor whose lines do not start on 16-byte boundaries, which TMA cannot
+// address, is first copied to lines that do.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "matmul.h"
+#include "partial_rows.cuh"
+#include "tcgen05_dev.cuh"
+#include "trace.h"
+#include "../../include/musa_plugin_kernels.h"
+
+namespace musa_b200 {
+namespace {
+
+// Set by a kernel whose wait ran out (see BarWait); read by MusaMatMulStatus.
+__device__ int g_status;
+
+// ------------------------------------------------------------- activations --
+
+// The 16-bit outputs keep 8 or 11 bits, the hardware exp2 and reciprocal are good to
+// about 2^-22.
+__device__ __forceinline__ float SigmoidOf(float z) {
+  return __fdividef(1.0f, 1.0f + __expf(-z));
+}
+__device__ __forceinline__ float NormalCdf(float z) {
+  return fmaf(0.5f, erff(z * 0.70710678f), 0.5f);
+}
+
+template <int kN>
+__device__ __forceinline__ void Activate(float (&v)[kN], int act) {
+  switch (act) {
+    case MUSA_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];  // NaN goes through
+      break;
+    case MUSA_ACT_SIGMOID:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) v[i] = SigmoidOf(v[i]);
+      break;
+    case MUSA_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) v[i] *= SigmoidOf(v[i]);
+      break;
+    case MUSA_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) v[i] *= NormalCdf(v[i]);
+      break;
+    default:
+      break;
+  }
+}
+
+// act'(z)
+__device__ __forceinline__ float Slope(float z, int act) {
+  switch (act) {
+    case MUSA_ACT_RELU:
+      return z > 0.0f ? 1.0f : 0.0f;
+    case MUSA_ACT_SIGMOID: {
+      const float p = SigmoidOf(z);
+      return p * (1.0f - p);
+    }
+    case MUSA_ACT_SILU: {
+      const float p = SigmoidOf(z);
+      return p * fmaf(z, 1.0f - p, 1.0f);
+    }
+    case MUSA_ACT_GELU:
+      return fmaf(z * 0.39894228f, __expf(-0.5f * z * z), NormalCdf(z));
+    default:
+      return 1.0f;
+  }
+}
+
+// -------------------------------------------------------- products, any size --
+
+// Tiles of 128 columns of the product (lanes of tensor memory) x `rows_tile` rows of it
+// (columns of tensor memory).  The product is computed transposed: what is stored for one
+// row of it by the 32 lanes of a warp is contiguous whatever n, alignment and pitch, and
+// a product of few rows (decoding) asks for no more than it has: the weights are the
+// instruction's 128-row side, the rows its 16 .. 256-column side.  A reduction is
+// split over the CTAs of a cluster when the tiles alone do not fill the machine; their
+// partial tiles meet in shared memory (each CTA adds, in rank order, and finishes its
+// share of the rows), so there is no scratch, no second launch and no atomic.
+constexpr int kDepthBytes = 128;    // of both factors per stage
+constexpr int kSideBytes = 128 * kDepthBytes;
+constexpr int kMaxStages = 12;
+constexpr int kSplitThreads = 192;  // four warps for the epilogue, one for TMA, one for the MMA
+
+struct SplitArgs {
+  Epilogue e;
+  int64_t m, n;
+  int blocks;      // stages of depth in all
+  int rows_tile;
+  int stages;
+  int stage_bytes;
+  int splits;      // CTAs of the cluster
+  uint32_t idesc;
+  uint32_t tmem_columns;
+  bool p_rows, q_rows;   // the factors' rows_contiguous
+};
+
+__device__ __forceinline__ float LoadClusterF32At(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Rows row .. row + kN - 1 of the product in column `col`: one value per lane and row.
+template <typename T, int kN>
+__device__ __forceinline__ void FinishColumn(float (&v)[kN], int64_t row, int64_t col,
+                                             const SplitArgs& a, float bias, float col_scale) {
+  const Epilogue& e = a.e;
+  const bool inside = col < a.n;
+  T* y = static_cast<T*>(e.y) + row * a.n + col;
+  const int rows = a.m - row < kN ? static_cast<int>(a.m - row) : kN;
+  float r[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) r[i] = 0.0f;
+  if (e.residual != nullptr) {
+    const T* at = static_cast<const T*>(e.residual) + row * a.n + col;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      if (inside && i < rows) r[i] = ToF32(at[i * a.n]);
+    }
+  }
+  if (e.a_scale != nullptr) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      if (i < rows) v[i] *= e.a_scale[row + i] * col_scale;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kN; ++i) v[i] += bias;
+  if (e.z != nullptr) {
+    T* z = static_cast<T*>(e.z) + row * a.n + col;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      if (inside && i < rows) z[i * a.n] = FromF32<T>(v[i]);
+    }
+  }
+  Activate(v, e.act);
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    if (inside && i < rows) y[i * a.n] = FromF32<T>(v[i] + r[i]);
+  }
+}
+
+// P: the factor of the product's columns (b), Q: that of its rows (a).
+template <typename T, bool kBytes>
+__global__ void __launch_bounds__(kSplitThreads)
+    SplitProductKernel(const __grid_constant__ CUtensorMap p_map,
+                       const __grid_constant__ CUtensorMap q_map,
+                       const __grid_constant__ SplitArgs a) {
+  extern __shared__ uint8_t dynamic[];
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done;
+  __shared__ uint32_t tmem_at;
+  __shared__ volatile int give_up;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t ring = (SmemAddr(dynamic) + 1023u) & ~1023u;
+  const uint32_t rank = a.splits > 1 ? ClusterCtaRank() : 0;
+  const int64_t col0 = static_cast<int64_t>(blockIdx.x) * 128;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * a.rows_tile;
+  const int first = static_cast<int>(static_cast<int64_t>(a.blocks) * rank / a.splits);
+  const int last = static_cast<int>(static_cast<int64_t>(a.blocks) * (rank + 1) / a.splits);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      BarInit(SmemAddr(&full[s]), 1);
+      BarInit(SmemAddr(&empty[s]), 1);
+    }
+    BarInit(SmemAddr(&done), 1);
+    give_up = 0;
+    BarInitFence();
+  }
+  if (warp == 5) TmemAlloc<1>(SmemAddr(&tmem_at), a.tmem_columns);
+  TmemFenceBefore();
+  __syncthreads();
+  TmemFenceAfter();
+  const uint32_t tmem = tmem_at;
+  bool ok = true;
+
+  if (warp == 4 && lane == 0) {
+    constexpr int kDepth = kBytes ? kDepthBytes : kDepthBytes / 2;  // elements
+    for (int i = 0; i < last - first; ++i) {
+      const int s = i % a.stages;
+      if (!BarWait(SmemAddr(&empty[s]), ((i / a.stages) & 1) ^ 1, &give_up, &g_status)) {
+        ok = false;
+        break;
+      }
+      const uint32_t bar = SmemAddr(&full[s]);
+      const uint32_t p = ring + s * a.stage_bytes, q = p + kSideBytes;
+      const int depth = (first + i) * kDepth;
+      BarExpect(bar, a.stage_bytes);
+      if (a.p_rows) {
+        for (int b = 0; b < 2; ++b) {
+          TmaLoad<false>(p + b * kBlockBytes, &p_map, static_cast<int>(col0) + b * 64, depth, bar);
+        }
+      } else {
+        TmaLoad<false>(p, &p_map, depth, static_cast<int>(col0), bar);
+      }
+      if (a.q_rows) {
+        for (int b = 0; b < a.rows_tile / 64; ++b) {
+          TmaLoad<false>(q + b * kBlockBytes, &q_map, static_cast<int>(row0) + b * 64, depth, bar);
+        }
+      } else {
+        TmaLoad<false>(q, &q_map, depth, static_cast<int>(row0), bar);
+      }
+    }
+  } else if (warp == 5 && lane == 0) {
+    const uint32_t p_step = DepthStep(a.p_rows), q_step = DepthStep(a.q_rows);
+    for (int i = 0; i < last - first; ++i) {
+      const int s = i % a.stages;
+      if (!BarWait(SmemAddr(&full[s]), (i / a.stages) & 1, &give_up, &g_status)) {
+        ok = false;
+        break;
+      }
+      TmemFenceAfter();
+      const uint32_t p = ring + s * a.stage_bytes;
+      const uint64_t pd = OperandDesc(p, a.p_rows), qd = OperandDesc(p + kSideBytes, a.q_rows);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        Mma<1, kBytes>(tmem, pd + j * p_step, qd + j * q_step, a.idesc, i > 0 || j > 0);
+      }
+      MmaCommit<1>(SmemAddr(&empty[s]));
+    }
+    if (ok && last > first) MmaCommit<1>(SmemAddr(&done));
+  }
+  __syncwarp();
+  if (warp < 4 && last > first) {
+    ok = BarWait(SmemAddr(&done), 0, &give_up, &g_status);
+    TmemFenceAfter();
+  }
+  const int64_t col = col0 + warp * 32 + lane;
+  float bias = 0.0f, col_scale = 1.0f;
+  if (warp < 4 && col < a.n) {
+    if (a.e.bias != nullptr) bias = ToF32(static_cast<const T*>(a.e.bias)[col]);
+    if (a.e.b_scale != nullptr) col_scale = a.e.b_scale[col];
+  }
+  const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
+  if (a.splits == 1) {
+    if (warp < 4 && ok) {
+      for (int c = 0; c < a.rows_tile && row0 + c < a.m; c += 16) {
+        float v[16];
+        if (last > first) {
+          TmemLoad(lanes + c, v);
+          TmemLoadWait(v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+        }
+        FinishColumn<T>(v, row0 + c, col, a, bias, col_scale);
+      }
+    }
+  } else {
+    // Partial tile [row][128 columns] over the ring: this CTA's copies and matrix
+    // instructions are done.
+    if (warp < 4 && ok) {
+      for (int c = 0; c < a.rows_tile; c += 16) {
+        float v[16];
+        TmemLoad(lanes + c, v);
+        TmemLoadWait(v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + ((c + i) * 128 + warp * 32 + lane) * 4),
+                       "f"(v[i])
+                       : "memory");
+        }
+      }
+    }
+    ClusterSync();
+    if (warp < 4 && ok) {
+      const int share = a.rows_tile / a.splits;
+      for (int c = 0; c < share; c += 2) {
+        const int row = static_cast<int>(rank) * share + c;
+        float v[2] = {0.0f, 0.0f};
+        for (int s = 0; s < a.splits; ++s) {
+          const uint32_t at = MapToCta(ring + (row * 128 + warp * 32 + lane) * 4, s);
+          v[0] += LoadClusterF32At(at);
+          v[1] += LoadClusterF32At(at + 512);
+        }
+        if (row0 + row < a.m) FinishColumn<T>(v, row0 + row, col, a, bias, col_scale);
+      }
+    }
+    ClusterSync();
+  }
+  TmemFenceBefore();
+  __syncthreads();
+  if (give_up != 0) LeaveInFlight();
+  if (warp == 5) {
+    TmemFenceAfter();
+    TmemFree<1>(tmem, a.tmem_columns);
+  }
+}
+
+// ---------------------------------------------------------------- factors --
+
+// Lines of `columns` elements, `ld` apart, to lines `pitch` apart.
+template <typename E>
+__global__ void __launch_bounds__(256)
+    RepitchKernel(const E* __restrict__ src, E* __restrict__ dst, int64_t lines, int64_t columns,
+                  int64_t ld, int64_t pitch) {
+  for (int64_t r = blockIdx.y; r < lines; r += gridDim.y) {
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (c + i * 256 < columns) dst[r * pitch + c + i * 256] = src[r * ld + c + i * 256];
+    }
+  }
+}
+
+int64_t RoundUp(int64_t v, int64_t to) { return CeilDiv(v, to) * to; }
+
+// A factor's lines in memory.
+struct Lines {
+  int64_t count, length;
+};
+Lines LinesOf(const Factor& f, int64_t rows, int64_t depth) {
+  return f.rows_contiguous ? Lines{depth, rows} : Lines{rows, depth};
+}
+
+// TMA takes it as it lies: 16-byte aligned base and lines.
+bool Addressable(const Factor& f, const Lines& l, int elem) {
+  return Aligned16(f.p) && (l.count <= 1 || f.ld * elem % 16 == 0);
+}
+
+size_t RepitchBytes(const Factor& f, int64_t rows, int64_t depth, int elem) {
+  const Lines l = LinesOf(f, rows, depth);
+  // Lines of 8-bit factors have to run along the depth.
+  if (l.count == 0 || l.length == 0 || Addressable(f, l, elem)) return 0;
+  return static_cast<size_t>(RoundUp(l.length * elem, 16) * l.count + 16);
+}
+
+cudaError_t Repitch(Factor* f, int64_t rows, int64_t depth, int elem, uint8_t** workspace,
+                    cudaStream_t stream) {
+  const size_t bytes = RepitchBytes(*f, rows, depth, elem);
+  if (bytes == 0) return cudaSuccess;
+  const Lines l = LinesOf(*f, rows, depth);
+  const int64_t pitch = RoundUp(l.length * elem, 16) / elem;
+  const dim3 grid(static_cast<unsigned>(CeilDiv(l.length, 1024)),
+                  static_cast<unsigned>(l.count < 32768 ? l.count : 32768));
+  CountKernelLaunch();
+  if (elem == 2) {
+    RepitchKernel<uint16_t><<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(f->p),
+                                                      reinterpret_cast<uint16_t*>(*workspace),
+                                                      l.count, l.length, f->ld, pitch);
+  } else {
+    RepitchKernel<uint8_t><<<grid, 256, 0, stream>>>(static_cast<const uint8_t*>(f->p),
+                                                     *workspace, l.count, l.length, f->ld, pitch);
+  }
+  f->p = *workspace;
+  f->ld = pitch;
+  *workspace += RoundUp(static_cast<int64_t>(bytes), 16);
+  return cudaGetLastError();
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                              const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn Encode() {
+  static const EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
+                                         &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return static_cast<EncodeFn>(nullptr);
+    }
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+// A map over lines of memory with boxes of 128 bytes x `box_lines`, swizzled.
+template <typename T>
+constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+template <>
+constexpr CUtensorMapDataType kMapType<__half> = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+template <>
+constexpr CUtensorMapDataType kMapType<__nv_bfloat16> = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+
+template <typename E>
+bool MakeMap(CUtensorMap* map, const void* p, int64_t count, int64_t length, int64_t ld,
+             int box_lines) {
+  const EncodeFn encode = Encode();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(length), static_cast<cuuint64_t>(count)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(
+      count > 1 ? ld * static_cast<int64_t>(sizeof(E)) : RoundUp(length * sizeof(E), 16))};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / sizeof(E)),
+                             static_cast<cuuint32_t>(box_lines)};
+  const cuuint32_t steps[2] = {1, 1};
+  return encode(map, kMapType<E>, 2, const_cast<void*>(p), dims, strides, box, steps,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// ---------------------------------------------------------------- launches --
+
+template <typename T, bool kBytes>
+int LaunchSplit(int64_t m, int64_t n, int64_t k, const Factor& fa, const Factor& fb,
+                const Epilogue& e, cudaStream_t stream) {
+  using E = std::conditional_t<kBytes, uint8_t, T>;
+  constexpr int kDepth = 128 / sizeof(E);
+  SplitArgs a = {};
+  a.e = e;
+  a.m = m;
+  a.n = n;
+  a.blocks = static_cast<int>(CeilDiv(k, kDepth));
+  a.p_rows = fb.rows_contiguous;
+  a.q_rows = fa.rows_contiguous;
+  a.rows_tile = static_cast<int>(m >= 256 ? 256 : RoundUp(m, a.q_rows ? 64 : 16));
+  a.stage_bytes = kSideBytes + a.rows_tile * kDepthBytes;
+  // Two CTAs per SM where four stages fit half an SM's shared memory.
+  const int budget = a.stage_bytes * 4 <= 104 * 1024 ? 104 * 1024 : 208 * 1024;
+  a.stages = budget / a.stage_bytes;
+  if (a.stages > kMaxStages) a.stages = kMaxStages;
+  const int64_t tiles = CeilDiv(n, 128) * CeilDiv(m, a.rows_tile);
+  const int64_t slots = static_cast<int64_t>(SmCount()) * (budget < 128 * 1024 ? 2 : 1);
+  a.splits = 1;
+  while (a.splits < 8 && tiles * a.splits * 2 <= slots && a.blocks >= a.splits * 2 * 2) {
+    a.splits *= 2;
+  }
+  a.tmem_columns = 32;
+  while (a.tmem_columns < static_cast<uint32_t>(a.rows_tile)) a.tmem_columns *= 2;
+  constexpr int kType = kBytes ? 0 : std::is_same_v<T, __nv_bfloat16> ? 1 : 0;
+  a.idesc = InstructionDesc(kType, a.p_rows, a.q_rows, 128, a.rows_tile);
+  CUtensorMap p_map, q_map;
+  const Lines pl = LinesOf(fb, n, k), ql = LinesOf(fa, m, k);
+  if (k > 0 && (!MakeMap<E>(&p_map, fb.p, pl.count, pl.length, fb.ld, a.p_rows ? 64 : 128) ||
+                !MakeMap<E>(&q_map, fa.p, ql.count, ql.length, fa.ld,
+                            a.q_rows ? 64 : a.rows_tile))) {
+    return MUSA_KERNELS_EINVAL;
+  }
+  const int smem = a.stages * a.stage_bytes + 1024;
+  static std::atomic<int> ready[kMaxDevices];
+  PerDevice(ready, [] {
+    return cudaFuncSetAttribute(SplitProductKernel<T, kBytes>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                210 * 1024) == cudaSuccess
+               ? 1
+               : 0;
+  });
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(CeilDiv(n, 128)),
+                     static_cast<unsigned>(CeilDiv(m, a.rows_tile)),
+                     static_cast<unsigned>(a.splits));
+  cfg.blockDim = dim3(kSplitThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = static_cast<unsigned>(a.splits);
+  cfg.attrs = attr;
+  cfg.numAttrs = a.splits > 1 ? 1 : 0;
+  CountKernelLaunch();
+  return static_cast<int>(
+      cudaLaunchKernelEx(&cfg, SplitProductKernel<T, kBytes>, p_map, q_map, a));
+}
+
+template <typename T, bool kBytes>
+int Product(int64_t m, int64_t n, int64_t k, const Factor& fa, const Factor& fb,
+            const Epilogue& e, cudaStream_t stream) {
+  return LaunchSplit<T, kBytes>(m, n, k, fa, fb, e, stream);
+}
+
+// ---------------------------------------------------------------- gradient --
+
+// dz = dy * act'(z), rounded to the factors' type (what the tensor cores multiply), and the
+// column sums of the unrounded dz: CTA (x, y) walks a range of rows of a block of columns and
+// leaves one fp32 partial row; the partial rows are added in order.
+constexpr int kSumRows = 8;      // row lanes of a CTA
+
+struct SlopeArgs {
+  const void* dy;
+  const void* z;
+  void* dz;          // null: not wanted (dy itself serves)
+  float* partial;    // [gridDim.y][n]
+  int64_t m, n, pitch;
+  int64_t rows_per_cta;
+  int act;
+};
+
+template <typename T, int kVec>
+__global__ void __launch_bounds__(32 * kSumRows) SlopeKernel(SlopeArgs a) {
+  using P = Pack<T, kVec>;
+  __shared__ float sums[kSumRows][32 * kVec + 1];
+  const int lane = threadIdx.x % 32, row_lane = threadIdx.x / 32;
+  const int64_t col = (static_cast<int64_t>(blockIdx.x) * 32 + lane) * kVec;
+  const int64_t begin = blockIdx.y * a.rows_per_cta;
+  const int64_t end = begin + a.rows_per_cta < a.m ? begin + a.rows_per_cta : a.m;
+  float sum[kVec];
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) sum[e] = 0.0f;
+  if (col < a.n) {
+    const T* dy = static_cast<const T*>(a.dy) + col;
+    const T* z = static_cast<const T*>(a.z) + col;
+    T* dz = static_cast<T*>(a.dz) + col;
+#pragma unroll 4
+    for (int64_t r = begin + row_lane; r < end; r += kSumRows) {
+      const P g = *reinterpret_cast<const P*>(dy + r * a.n);
+      P out;
+      if (a.act != MUSA_ACT_IDENTITY) {
+        const P x = *reinterpret_cast<const P*>(z + r * a.n);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          const float d = ToF32(g.v[e]) * Slope(ToF32(x.v[e]), a.act);
+          sum[e] += d;
+          out.v[e] = FromF32<T>(d);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          sum[e] += ToF32(g.v[e]);
+          out.v[e] = g.v[e];
+        }
+      }
+      if (a.dz != nullptr) *reinterpret_cast<P*>(dz + r * a.pitch) = out;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) sums[row_lane][lane * kVec + e] = sum[e];
+  __syncthreads();
+  for (int c = threadIdx.x; c < 32 * kVec; c += 32 * kSumRows) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 32 * kVec + c;
+    float t = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kSumRows; ++r) t += sums[r][c];
+    if (at < a.n) a.partial[blockIdx.y * a.n + at] = t;
+  }
+}
+
+struct SumShape {
+  int64_t rows_per_cta;
+  int parts;
+};
+// About four CTAs per SM over columns and rows, at least 64 rows each.
+SumShape SumRows(int64_t m, int64_t n) {
+  const int64_t blocks = n > 0 ? CeilDiv(n, 256) : 1;
+  int64_t parts = CeilDiv(4 * 148, blocks);
+  if (parts > CeilDiv(m, 64)) parts = CeilDiv(m, 64);
+  if (parts < 1) parts = 1;
+  if (parts > 1024) parts = 1024;
+  const int64_t rows = CeilDiv(CeilDiv(m, parts), kSumRows) * kSumRows;
+  return {rows < 1 ? 1 : rows, static_cast<int>(rows < 1 ? 1 : CeilDiv(m, rows))};
+}
+
+struct GradPlan {
+  bool want_dz;        // dz goes to the workspace
+  int64_t dz_pitch;
+  SumShape sum;
+  size_t dz_bytes, partial_bytes, a_bytes, b_bytes;
+  size_t Total() const { return dz_bytes + partial_bytes + a_bytes + b_bytes + 64; }
+};
+
+GradPlan PlanGrad(const void* dy, const Factor& a, const Factor& b, int64_t m, int64_t n,
+                  int64_t k, int act) {
+  GradPlan p = {};
+  const bool direct = act == MUSA_ACT_IDENTITY && Aligned16(dy) && n % 8 == 0;
+  p.want_dz = !direct;
+  p.dz_pitch = RoundUp(n, 8);
+  p.sum = SumRows(m, n);
+  p.dz_bytes = p.want_dz ? static_cast<size_t>(RoundUp(p.dz_pitch * m * 2, 16)) : 0;
+  p.partial_bytes = static_cast<size_t>(RoundUp(n * p.sum.parts * 4, 16));
+  p.a_bytes = static_cast<size_t>(RoundUp(RepitchBytes(a, m, k, 2), 16));
+  p.b_bytes = static_cast<size_t>(RoundUp(RepitchBytes(b, n, k, 2), 16));
+  return p;
+}
+
+bool BadSizes(int64_t m, int64_t n, int64_t k) { return m < 0 || n < 0 || k < 0; }
+
+// grid.y holds the tiles of 256 rows; in a gradient every size is the rows of a product.
+bool TooLarge(int64_t m, int64_t n, int64_t k) {
+  constexpr int64_t kMost = int64_t(65535) * 256;
+  return m > kMost || n > kMost || k > kMost;
+}
+
+bool BadFactor(const Factor& f, int64_t rows, int64_t depth) {
+  const Lines l = LinesOf(f, rows, depth);
+  return l.count > 0 && l.length > 0 && (f.p == nullptr || (l.count > 1 && f.ld < l.length));
+}
+
+bool KnownAct(int act) {
+  return act == MUSA_ACT_IDENTITY || act == MUSA_ACT_RELU || act == MUSA_ACT_SIGMOID ||
+         act == MUSA_ACT_SILU || act == MUSA_ACT_GELU;
+}
+
+bool BadWorkspace(const void* workspace, size_t bytes, size_t need) {
+  return need > 0 && (workspace == nullptr || bytes < need || !Aligned16(workspace));
+}
+
+template <typename T>
+int Forward(Factor a, Factor b, const Epilogue& e, int64_t m, int64_t n, int64_t k,
+            void* workspace, size_t bytes, cudaStream_t stream) {
+  if (BadWorkspace(workspace, bytes, RepitchBytes(a, m, k, 2) + RepitchBytes(b, n, k, 2))) {
+    return MUSA_KERNELS_EWORKSPACE;
+  }
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  cudaError_t rc = Repitch(&a, m, k, 2, &ws, stream);
+  if (rc == cudaSuccess) rc = Repitch(&b, n, k, 2, &ws, stream);
+  return rc != cudaSuccess ? static_cast<int>(rc)
+                           : Product<T, false>(m, n, k, a, b, e, stream);
+}
+
+template <typename T>
+int Backward(const void* dy, Factor a, Factor b, const void* z, void* da, void* db, void* dbias,
+             int64_t m, int64_t n, int64_t k, int act, void* workspace, size_t bytes,
+             cudaStream_t stream) {
+  const GradPlan p = PlanGrad(dy, a, b, m, n, k, act);
+  if (BadWorkspace(workspace, bytes, p.Total())) return MUSA_KERNELS_EWORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  float* partial = reinterpret_cast<float*>(ws);
+  ws += p.partial_bytes;
+  void* dz = p.want_dz ? ws : nullptr;
+  ws += p.dz_bytes;
+  cudaError_t rc = cudaSuccess;
+  if (m > 0 && n > 0) {
+    if (p.want_dz || dbias != nullptr) {
+      SlopeArgs s = {dy, z, dz, partial, m, n, p.dz_pitch, p.sum.rows_per_cta, act};
+      const bool packed = n % 8 == 0 && Aligned16(dy) && (z == nullptr || Aligned16(z));
+      const dim3 grid(static_cast<unsigned>(CeilDiv(n, packed ? 256 : 32)),
+                      static_cast<unsigned>(p.sum.parts));
+      CountKernelLaunch();
+      if (packed) SlopeKernel<T, 8><<<grid, 32 * kSumRows, 0, stream>>>(s);
+      else SlopeKernel<T, 1><<<grid, 32 * kSumRows, 0, stream>>>(s);
+      if (dbias != nullptr) {
+        rc = LaunchAddPartialRows<T>(false, partial, p.sum.parts, n, dbias, stream);
+        if (rc != cudaSuccess) return static_cast<int>(rc);
+      }
+    }
+  } else if (dbias != nullptr && n > 0) {
+    cudaMemsetAsync(dbias, 0, sizeof(T) * n, stream);
+  }
+  rc = cudaGetLastError();
+  if (rc == cudaSuccess && db != nullptr && m > 0) rc = Repitch(&a, m, k, 2, &ws, stream);
+  if (rc == cudaSuccess && da != nullptr && n > 0) rc = Repitch(&b, n, k, 2, &ws, stream);
+  if (rc != cudaSuccess) return static_cast<int>(rc);
+  const void* g = p.want_dz ? dz : dy;
+  const int64_t ldg = p.want_dz ? p.dz_pitch : n;
+  int code = MUSA_KERNELS_OK;
+  Epilogue e = {};
+  if (da != nullptr && m > 0 && k > 0) {
+    e.y = da;
+    // op(b) read along n.
+    const Factor ob = {b.p, b.ld, !b.rows_contiguous};
+    code = a.rows_contiguous
+               ? Product<T, false>(k, m, n, ob, Factor{g, ldg, false}, e, stream)
+               : Product<T, false>(m, k, n, Factor{g, ldg, false}, ob, e, stream);
+    if (code != MUSA_KERNELS_OK) return code;
+  }
+  if (db != nullptr && n > 0 && k > 0) {
+    e.y = db;
+    const Factor oa = {a.p, a.ld, !a.rows_contiguous};
+    code = b.rows_contiguous
+               ? Product<T, false>(k, n, m, oa, Factor{g, ldg, true}, e, stream)
+               : Product<T, false>(n, k, m, Factor{g, ldg, true}, oa, e, stream);
+  }
+  return code;
+}
+
+}  // namespace
+}  // namespace musa_b200
+
+using namespace musa_b200;
+
+extern "C" {
+
+int MusaMatMulStatus(void) {
+  int v = 0;
+  const cudaError_t rc = cudaMemcpyFromSymbol(&v, g_status, sizeof(v));
+  return rc != cudaSuccess ? static_cast<int>(rc) : v == 0 ? MUSA_KERNELS_OK : MUSA_KERNELS_EGAVEUP;
+}
+
+size_t MatMulWorkspaceBytes(int elem_bytes, const void* a, int64_t lda, bool transpose_a,
+                            const void* b, int64_t ldb, bool transpose_b, int64_t m, int64_t n,
+                            int64_t k) {
+  if (BadSizes(m, n, k) || (elem_bytes != 1 && elem_bytes != 2)) return 0;
+  return RepitchBytes(Factor{a, lda, transpose_a}, m, k, elem_bytes) +
+         RepitchBytes(Factor{b, ldb, !transpose_b}, n, k, elem_bytes);
+}
+
+int LaunchMatMulBiasAct(int dtype, const void* a, int64_t lda, bool transpose_a, const void* b,
+                        int64_t ldb, bool transpose_b, const void* bias, const void* residual,
+                        void* y, void* preactivation, int64_t m, int64_t n, int64_t k, int act,
+                        void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  if (dtype != MUSA_DT_F16 && dtype != MUSA_DT_BF16) return MUSA_KERNELS_EUNSUPPORTED;
+  if (!KnownAct(act)) return MUSA_KERNELS_EUNSUPPORTED;
+  if (BadSizes(m, n, k)) return MUSA_KERNELS_EINVAL;
+  if (TooLarge(m, n, k)) return MUSA_KERNELS_ETOOLARGE;
+  const int outputs = 1 + (preactivation != nullptr) + (residual != nullptr);
+  MUSA_TRACE("LaunchMatMulBiasAct", 2 * (m * k + k * n + outputs * m * n));
+  if (m == 0 || n == 0) return MUSA_KERNELS_OK;
+  const Factor fa = {a, lda, transpose_a}, fb = {b, ldb, !transpose_b};
+  if (y == nullptr || BadFactor(fa, m, k) || BadFactor(fb, n, k)) return MUSA_KERNELS_EINVAL;
+  const Epilogue e = {bias, residual, nullptr, nullptr, y, preactivation, act};
+  return dtype == MUSA_DT_F16
+             ? Forward<__half>(fa, fb, e, m, n, k, workspace, workspace_bytes, stream)
+             : Forward<__nv_bfloat16>(fa, fb, e, m, n, k, workspace, workspace_bytes, stream);
+}
+
+size_t MatMulGradWorkspaceBytes(const void* dy, const void* a, int64_t lda, bool transpose_a,
+                                const void* b, int64_t ldb, bool transpose_b, int64_t m,
+                                int64_t n, int64_t k, int act) {
+  if (BadSizes(m, n, k)) return 0;
+  return PlanGrad(dy, Factor{a, lda, transpose_a}, Factor{b, ldb, !transpose_b}, m, n, k, act)
+      .Total();
+}
+
+int LaunchMatMulBiasActGrad(int dtype, const void* dy, const void* a, int64_t lda,
+                            bool transpose_a, const void* b, int64_t ldb, bool transpose_b,
+                            const void* preactivation, void* da, void* db, void* dbias, int64_t m,
+                            int64_t n, int64_t k, int act, void* workspace,
+                            size_t workspace_bytes, cudaStream_t stream) {
+  if (dtype != MUSA_DT_F16 && dtype != MUSA_DT_BF16) return MUSA_KERNELS_EUNSUPPORTED;
+  if (!KnownAct(act)) return MUSA_KERNELS_EUNSUPPORTED;
+  if (BadSizes(m, n, k)) return MUSA_KERNELS_EINVAL;
+  if (TooLarge(m, n, k)) return MUSA_KERNELS_ETOOLARGE;
+  MUSA_TRACE("LaunchMatMulBiasActGrad",
+             2 * ((act == MUSA_ACT_IDENTITY ? 1 : 2) * m * n + 2 * m * k + 2 * k * n));
+  const Factor fa = {a, lda, transpose_a}, fb = {b, ldb, !transpose_b};
+  if (BadFactor(fa, m, k) || BadFactor(fb, n, k)) return MUSA_KERNELS_EINVAL;
+  if (m > 0 && n > 0 &&
+      (dy == nullptr || (act != MUSA_ACT_IDENTITY && preactivation == nullptr))) {
+    return MUSA_KERNELS_EINVAL;
+  }
+  return dtype == MUSA_DT_F16
+             ? Backward<__half>(dy, fa, fb, preactivation, da, db, dbias, m, n, k, act, workspace,
+                                workspace_bytes, stream)
+             : Backward<__nv_bfloat16>(dy, fa, fb, preactivation, da, db, dbias, m, n, k, act,
+                                       workspace, workspace_bytes, stream);
+}
+
+int LaunchQuantizedMatMulBiasAct(int out_dtype, const void* a, int64_t lda, const float* a_scale,
+                                 const void* b, int64_t ldb, const float* b_scale,
+                                 const void* bias, const void* residual, void* y, int64_t m,
+                                 int64_t n, int64_t k, int act, void* workspace,
+                                 size_t workspace_bytes, cudaStream_t stream) {
+  if (out_dtype != MUSA_DT_F16 && out_dtype != MUSA_DT_BF16) return MUSA_KERNELS_EUNSUPPORTED;
+  if (!KnownAct(act)) return MUSA_KERNELS_EUNSUPPORTED;
+  if (BadSizes(m, n, k)) return MUSA_KERNELS_EINVAL;
+  if (TooLarge(m, n, k)) return MUSA_KERNELS_ETOOLARGE;
+  MUSA_TRACE("LaunchQuantizedMatMulBiasAct",
+             m * k + k * n + 2 * (residual != nullptr ? 2 : 1) * m * n);
+  if (m == 0 || n == 0) return MUSA_KERNELS_OK;
+  Factor fa = {a, lda, false}, fb = {b, ldb, false};
+  if (y == nullptr || a_scale == nullptr || b_scale == nullptr || BadFactor(fa, m, k) ||
+      BadFactor(fb, n, k)) {
+    return MUSA_KERNELS_EINVAL;
+  }
+  if (BadWorkspace(workspace, workspace_bytes,
+                   RepitchBytes(fa, m, k, 1) + RepitchBytes(fb, n, k, 1))) {
+    return MUSA_KERNELS_EWORKSPACE;
+  }
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  cudaError_t rc = Repitch(&fa, m, k, 1, &ws, stream);
+  if (rc == cudaSuccess) rc = Repitch(&fb, n, k, 1, &ws, stream);
+  if (rc != cudaSuccess) return static_cast<int>(rc);
+  const Epilogue e = {bias, residual, a_scale, b_scale, y, nullptr, act};
+  return out_dtype == MUSA_DT_F16 ? Product<__half, true>(m, n, k, fa, fb, e, stream)
+                                  : Product<__nv_bfloat16, true>(m, n, k, fa, fb, e, stream);
+}
+
+}  // extern "C"

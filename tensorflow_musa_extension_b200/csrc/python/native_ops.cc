@@ -27,6 +27,8 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <cmath>
+#include <optional>
+#include <vector>
 
 #include "../../../include/musa_plugin_kernels.h"
 
@@ -42,7 +44,12 @@ struct Api {
   X(LaunchLayerNorm_BF16) X(LayerNormGradWorkspaceBytes) X(LaunchLayerNormGrad_F32)       \
   X(LaunchLayerNormGrad_F16) X(LaunchLayerNormGrad_BF16) X(LaunchRmsNormFloat)            \
   X(LaunchRmsNormBFloat16) X(LaunchRmsNormGradDxFloat) X(LaunchRmsNormGradDxBFloat16)     \
-  X(LaunchApplyAdamGroupHostTable)
+  X(LaunchApplyAdamGroupHostTable) X(LaunchAddRmsNorm_F32) X(LaunchAddRmsNorm_F16)        \
+  X(LaunchAddRmsNorm_BF16) X(AddRmsNormGradWorkspaceBytes) X(LaunchAddRmsNormGrad_F32)    \
+  X(LaunchAddRmsNormGrad_F16) X(LaunchAddRmsNormGrad_BF16) X(LaunchAddRmsNormQuantize_F32) \
+  X(LaunchAddRmsNormQuantize_F16) X(LaunchAddRmsNormQuantize_BF16) X(MatMulWorkspaceBytes) \
+  X(LaunchMatMulBiasAct) X(MatMulGradWorkspaceBytes) X(LaunchMatMulBiasActGrad)           \
+  X(LaunchQuantizedMatMulBiasAct)
 #define X(name) decltype(&::name) name = nullptr;
   MUSA_API(X)
 #undef X
@@ -463,6 +470,255 @@ PyObject* RmsNormGradDx(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// An optional tensor: `t` null for None; false where the launchers cannot take it as it is.
+bool Optional(PyObject* o, const at::Tensor** t) {
+  *t = o == Py_None ? nullptr : Direct(o);
+  return o == Py_None || *t != nullptr;
+}
+
+bool Like(const at::Tensor* t, const at::Tensor& x) {
+  return t != nullptr && t->scalar_type() == x.scalar_type() && t->sizes() == x.sizes() &&
+         t->device() == x.device();
+}
+
+void* Data(const at::Tensor* t) { return t == nullptr ? nullptr : t->data_ptr(); }
+
+// One fp32 value per row of x.
+std::vector<int64_t> RowShape(const at::Tensor& x) {
+  auto shape = x.sizes().vec();
+  shape.back() = 1;
+  return shape;
+}
+
+// x, residual, gamma, epsilon -> y, sum, inv_rms
+PyObject* AddRmsNorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4 || !NoModes()) Py_RETURN_NONE;
+  const at::Tensor *xp = Direct(a[0]), *r = Direct(a[1]), *g = Direct(a[2]);
+  double eps;
+  if (!xp || !Number(a[3], &eps) || xp->dim() < 1 || xp->numel() == 0) Py_RETURN_NONE;
+  const at::Tensor& x = *xp;
+  const int code = DtypeCode(x.scalar_type());
+  const int64_t last = x.size(-1);
+  if (code < 0 || !Like(r, x) || !RowVector(g, x, last)) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor y = EmptyLike(x), sum = EmptyLike(x), inv = Empty(RowShape(x), at::kFloat);
+  int rc;
+  {
+    pybind11::gil_scoped_release nogil;
+    rc = ByDtype(code, g_api.LaunchAddRmsNorm_F32, g_api.LaunchAddRmsNorm_F16,
+                 g_api.LaunchAddRmsNorm_BF16)(
+        x.data_ptr(), r->data_ptr(), g->data_ptr(), y.data_ptr(), sum.data_ptr(),
+        static_cast<float*>(inv.data_ptr()), x.numel() / last, last, static_cast<float>(eps),
+        StreamOf(x));
+  }
+  return Results(rc, {y, sum, inv});
+  END_HANDLE_TH_ERRORS
+}
+
+// dy, dsum, sum, inv_rms, gamma -> dx, dgamma
+PyObject* AddRmsNormGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || !NoModes()) Py_RETURN_NONE;
+  const at::Tensor *dy = Direct(a[0]), *ds, *sp = Direct(a[2]), *inv = Direct(a[3]);
+  const at::Tensor* g = Direct(a[4]);
+  if (!Optional(a[1], &ds) || !sp || sp->dim() < 1 || sp->numel() == 0) Py_RETURN_NONE;
+  const at::Tensor& s = *sp;
+  const int code = DtypeCode(s.scalar_type());
+  const int64_t last = s.size(-1), rows = s.numel() / last;
+  if (code < 0 || !Like(dy, s) || (ds != nullptr && !Like(ds, s)) || !RowVector(g, s, last) ||
+      inv == nullptr || inv->scalar_type() != at::kFloat || inv->numel() != rows ||
+      inv->device() != s.device()) {
+    Py_RETURN_NONE;
+  }
+  const c10::cuda::CUDAGuard guard(s.device());
+  at::Tensor dx = EmptyLike(s), dg = EmptyLike(*g);
+  int rc;
+  {
+    const Scratch ws(g_api.AddRmsNormGradWorkspaceBytes(rows, last));
+    pybind11::gil_scoped_release nogil;
+    rc = ByDtype(code, g_api.LaunchAddRmsNormGrad_F32, g_api.LaunchAddRmsNormGrad_F16,
+                 g_api.LaunchAddRmsNormGrad_BF16)(
+        dy->data_ptr(), Data(ds), s.data_ptr(), static_cast<const float*>(inv->data_ptr()),
+        g->data_ptr(), dx.data_ptr(), dg.data_ptr(), rows, last, ws.data.get(), ws.size,
+        StreamOf(s));
+  }
+  return Results(rc, {dx, dg});
+  END_HANDLE_TH_ERRORS
+}
+
+// x, residual or None, gamma or None, epsilon -> q, scale, sum or None
+PyObject* AddRmsNormQuantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4 || !NoModes()) Py_RETURN_NONE;
+  const at::Tensor *xp = Direct(a[0]), *r, *g;
+  double eps;
+  if (!xp || !Optional(a[1], &r) || !Optional(a[2], &g) || !Number(a[3], &eps)) Py_RETURN_NONE;
+  const at::Tensor& x = *xp;
+  const int code = DtypeCode(x.scalar_type());
+  if (code < 0 || x.dim() < 1 || x.numel() == 0) Py_RETURN_NONE;
+  const int64_t last = x.size(-1);
+  if ((r != nullptr && !Like(r, x)) || (g != nullptr && !RowVector(g, x, last))) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor q = Empty(x.sizes(), at::kFloat8_e4m3fn), scale = Empty(RowShape(x), at::kFloat);
+  at::Tensor sum;
+  if (r != nullptr) sum = EmptyLike(x);
+  int rc;
+  {
+    pybind11::gil_scoped_release nogil;
+    rc = ByDtype(code, g_api.LaunchAddRmsNormQuantize_F32, g_api.LaunchAddRmsNormQuantize_F16,
+                 g_api.LaunchAddRmsNormQuantize_BF16)(
+        x.data_ptr(), Data(r), Data(g), q.data_ptr(), static_cast<float*>(scale.data_ptr()),
+        sum.defined() ? sum.data_ptr() : nullptr, x.numel() / last, last,
+        static_cast<float>(eps), StreamOf(x));
+  }
+  return Results(rc, {q, scale, sum});
+  END_HANDLE_TH_ERRORS
+}
+
+// The sizes of a product of contiguous factors; false where they do not fit or are empty.
+struct ProductShape {
+  int64_t m, n, k, lda, ldb;
+  std::vector<int64_t> out;
+};
+bool ShapeOf(const at::Tensor& a, const at::Tensor& b, bool ta, bool tb, ProductShape* s) {
+  if (a.dim() < 2 || b.dim() != 2 || (ta && a.dim() != 2) || a.numel() == 0 || b.numel() == 0 ||
+      b.scalar_type() != a.scalar_type() || b.device() != a.device()) {
+    return false;
+  }
+  s->lda = a.size(-1);
+  s->ldb = b.size(1);
+  s->k = ta ? a.size(0) : s->lda;
+  s->m = a.numel() / s->k;
+  s->n = tb ? b.size(0) : b.size(1);
+  if ((tb ? b.size(1) : b.size(0)) != s->k) return false;
+  s->out = a.sizes().vec();
+  if (ta) s->out[0] = s->m;
+  s->out.back() = s->n;
+  return true;
+}
+
+bool Fits(const at::Tensor* t, at::IntArrayRef shape, at::ScalarType dtype,
+          const at::Tensor& like) {
+  return t == nullptr || (t->scalar_type() == dtype && t->sizes() == shape &&
+                          t->device() == like.device());
+}
+
+bool Half16(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
+
+// a, b, bias or None, residual or None, act, transpose_a, transpose_b,
+// return_preactivation -> y (, preactivation)
+PyObject* MatMulBiasAct(PyObject*, PyObject* const* o, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 8 || !NoModes() || !PyLong_CheckExact(o[4])) Py_RETURN_NONE;
+  const at::Tensor *ap = Direct(o[0]), *bp = Direct(o[1]), *bias, *res;
+  bool ta, tb, keep;
+  ProductShape s;
+  if (!ap || !bp || !Optional(o[2], &bias) || !Optional(o[3], &res) || !Flag(o[5], &ta) ||
+      !Flag(o[6], &tb) || !Flag(o[7], &keep) || !Half16(ap->scalar_type()) ||
+      !ShapeOf(*ap, *bp, ta, tb, &s)) {
+    Py_RETURN_NONE;
+  }
+  const at::Tensor &a = *ap, &b = *bp;
+  const at::ScalarType dtype = a.scalar_type();
+  if (!Fits(bias, {s.n}, dtype, a) || !Fits(res, s.out, dtype, a)) Py_RETURN_NONE;
+  const int act = static_cast<int>(PyLong_AsLong(o[4]));
+  const c10::cuda::CUDAGuard guard(a.device());
+  at::Tensor y = Empty(s.out, dtype), z;
+  if (keep) z = Empty(s.out, dtype);
+  int rc;
+  {
+    const size_t need = g_api.MatMulWorkspaceBytes(2, a.data_ptr(), s.lda, ta, b.data_ptr(),
+                                                   s.ldb, tb, s.m, s.n, s.k);
+    std::optional<Scratch> ws;
+    if (need > 0) ws.emplace(need);
+    pybind11::gil_scoped_release nogil;
+    rc = g_api.LaunchMatMulBiasAct(DtypeCode(dtype), a.data_ptr(), s.lda, ta, b.data_ptr(), s.ldb,
+                                   tb, Data(bias), Data(res), y.data_ptr(),
+                                   keep ? z.data_ptr() : nullptr, s.m, s.n, s.k, act,
+                                   ws ? ws->data.get() : nullptr, need, StreamOf(a));
+  }
+  if (keep) return Results(rc, {y, z});
+  return Results(rc, {y});
+  END_HANDLE_TH_ERRORS
+}
+
+// dy, a, b, preactivation or None, act, transpose_a, transpose_b -> da, db, dbias
+PyObject* MatMulBiasActGrad(PyObject*, PyObject* const* o, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 7 || !NoModes() || !PyLong_CheckExact(o[4])) Py_RETURN_NONE;
+  const at::Tensor *dy = Direct(o[0]), *ap = Direct(o[1]), *bp = Direct(o[2]), *z;
+  bool ta, tb;
+  ProductShape s;
+  if (!dy || !ap || !bp || !Optional(o[3], &z) || !Flag(o[5], &ta) || !Flag(o[6], &tb) ||
+      !Half16(ap->scalar_type()) || !ShapeOf(*ap, *bp, ta, tb, &s)) {
+    Py_RETURN_NONE;
+  }
+  const at::Tensor &a = *ap, &b = *bp;
+  const at::ScalarType dtype = a.scalar_type();
+  const int act = static_cast<int>(PyLong_AsLong(o[4]));
+  if (!Fits(dy, s.out, dtype, a) || !Fits(z, s.out, dtype, a) ||
+      (z == nullptr && act != MUSA_ACT_IDENTITY)) {
+    Py_RETURN_NONE;
+  }
+  const c10::cuda::CUDAGuard guard(a.device());
+  at::Tensor da = Empty(a.sizes(), dtype), db = Empty(b.sizes(), dtype), dbias = Empty(s.n, dtype);
+  int rc;
+  {
+    const Scratch ws(g_api.MatMulGradWorkspaceBytes(dy->data_ptr(), a.data_ptr(), s.lda, ta,
+                                                    b.data_ptr(), s.ldb, tb, s.m, s.n, s.k, act));
+    pybind11::gil_scoped_release nogil;
+    rc = g_api.LaunchMatMulBiasActGrad(DtypeCode(dtype), dy->data_ptr(), a.data_ptr(), s.lda, ta,
+                                       b.data_ptr(), s.ldb, tb, Data(z), da.data_ptr(),
+                                       db.data_ptr(), dbias.data_ptr(), s.m, s.n, s.k, act,
+                                       ws.data.get(), ws.size, StreamOf(a));
+  }
+  return Results(rc, {da, db, dbias});
+  END_HANDLE_TH_ERRORS
+}
+
+// a, a_scale, b, b_scale, bias or None, residual or None, act, out dtype code -> y
+PyObject* QuantizedMatMulBiasAct(PyObject*, PyObject* const* o, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  if (count != 8 || !NoModes() || !PyLong_CheckExact(o[6]) || !PyLong_CheckExact(o[7])) {
+    Py_RETURN_NONE;
+  }
+  const at::Tensor *ap = Direct(o[0]), *as = Direct(o[1]), *bp = Direct(o[2]);
+  const at::Tensor *bs = Direct(o[3]), *bias, *res;
+  const long code = PyLong_AsLong(o[7]);
+  ProductShape s;
+  if (!ap || !as || !bp || !bs || !Optional(o[4], &bias) || !Optional(o[5], &res) ||
+      (code != MUSA_DT_F16 && code != MUSA_DT_BF16) ||
+      ap->scalar_type() != at::kFloat8_e4m3fn || !ShapeOf(*ap, *bp, false, true, &s)) {
+    Py_RETURN_NONE;
+  }
+  const at::Tensor &a = *ap, &b = *bp;
+  const at::ScalarType dtype = code == MUSA_DT_F16 ? at::kHalf : at::kBFloat16;
+  if (!Fits(bias, {s.n}, dtype, a) || !Fits(res, s.out, dtype, a) ||
+      as->scalar_type() != at::kFloat || bs->scalar_type() != at::kFloat ||
+      as->numel() != s.m || bs->numel() != s.n || as->device() != a.device() ||
+      bs->device() != a.device()) {
+    Py_RETURN_NONE;
+  }
+  const int act = static_cast<int>(PyLong_AsLong(o[6]));
+  const c10::cuda::CUDAGuard guard(a.device());
+  at::Tensor y = Empty(s.out, dtype);
+  int rc;
+  {
+    const size_t need = g_api.MatMulWorkspaceBytes(1, a.data_ptr(), s.lda, false, b.data_ptr(),
+                                                   s.ldb, true, s.m, s.n, s.k);
+    std::optional<Scratch> ws;
+    if (need > 0) ws.emplace(need);
+    pybind11::gil_scoped_release nogil;
+    rc = g_api.LaunchQuantizedMatMulBiasAct(
+        static_cast<int>(code), a.data_ptr(), s.lda, static_cast<const float*>(as->data_ptr()),
+        b.data_ptr(), s.ldb, static_cast<const float*>(bs->data_ptr()), Data(bias), Data(res),
+        y.data_ptr(), s.m, s.n, s.k, act, ws ? ws->data.get() : nullptr, need, StreamOf(a));
+  }
+  return Results(rc, {y});
+  END_HANDLE_TH_ERRORS
+}
+
 // var, m, v, grad -> (device index, state code, grad code) as one number, or
 // -1: whether the update can share a launch with its neighbours.
 int AdamKind(PyObject* const* a) {
@@ -562,6 +818,12 @@ PyMethodDef kMethods[] = {
     {"layer_norm_grad", Fast(LayerNormGrad), METH_FASTCALL, nullptr},
     {"rms_norm", Fast(RmsNorm), METH_FASTCALL, nullptr},
     {"rms_norm_grad_dx", Fast(RmsNormGradDx), METH_FASTCALL, nullptr},
+    {"add_rms_norm", Fast(AddRmsNorm), METH_FASTCALL, nullptr},
+    {"add_rms_norm_grad", Fast(AddRmsNormGrad), METH_FASTCALL, nullptr},
+    {"add_rms_norm_quantize", Fast(AddRmsNormQuantize), METH_FASTCALL, nullptr},
+    {"matmul_bias_act", Fast(MatMulBiasAct), METH_FASTCALL, nullptr},
+    {"matmul_bias_act_grad", Fast(MatMulBiasActGrad), METH_FASTCALL, nullptr},
+    {"quantized_matmul_bias_act", Fast(QuantizedMatMulBiasAct), METH_FASTCALL, nullptr},
     {"adam_kind", Fast(AdamKindOf), METH_FASTCALL, nullptr},
     {"adam_group", Fast(AdamGroup), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -1,6 +1,11 @@
 """Op front end of the row normalisations: MusaLayerNorm, MusaLayerNormGrad,
 MusaRmsNorm, MusaRmsNormGradDx.  Same names, argument meaning, checks and error
-text as the reference ops; one launch each through the C ABI."""
+text as the reference ops; one launch each through the C ABI.
+
+New here, beyond the reference's ops: the residual's addition with the RMS norm
+behind it (MusaAddRmsNorm, MusaAddRmsNormGrad) and the same forward with an
+8-bit output (MusaAddRmsNormQuantize, MusaQuantizeRows), which the 8-bit
+product of linear_ops takes."""
 import collections
 
 import torch
@@ -15,6 +20,11 @@ MusaLayerNormGradOutput = collections.namedtuple(
     "MusaLayerNormGrad", ["dx", "dgamma", "dbeta"])
 MusaRmsNormOutput = collections.namedtuple(
     "MusaRmsNorm", ["y", "normalized", "inv_rms"])
+MusaAddRmsNormOutput = collections.namedtuple("MusaAddRmsNorm", ["y", "sum", "inv_rms"])
+MusaAddRmsNormGradOutput = collections.namedtuple("MusaAddRmsNormGrad", ["dx", "dgamma"])
+MusaAddRmsNormQuantizeOutput = collections.namedtuple(
+    "MusaAddRmsNormQuantize", ["q", "scale", "sum"])
+MusaQuantizeRowsOutput = collections.namedtuple("MusaQuantizeRows", ["q", "scale"])
 
 
 def _rows(x):
@@ -163,3 +173,130 @@ def MusaRmsNormGradDx(x, inv_rms, gamma, dy, name=None):
             fn(_r._ptr(xd), _r._ptr(inv.contiguous()), _r._ptr(g.contiguous()), _r._ptr(d),
                _r._ptr(dx), rows, last, _r._stream())
     return hf.back(dx)
+
+
+# ------------------------------------------ RMS norm of a residual's sum --
+
+def _check_rows(opname, x, others):
+    """x's rows and their length; `others`: (name, tensor, like x or a vector)."""
+    if x.dtype not in _LN_DTYPES:
+        raise InvalidArgumentError("%s: unsupported dtype %s" % (opname, x.dtype))
+    if x.dim() < 1:
+        raise InvalidArgumentError("Input rank must be >= 1")
+    rows, last = _rows(x)
+    for name, t, vector in others:
+        if t is None:
+            continue
+        if t.dtype != x.dtype:
+            raise InvalidArgumentError(
+                "%s: %s dtype %s does not match %s" % (opname, name, t.dtype, x.dtype))
+        if t.device != x.device:
+            raise InvalidArgumentError(
+                "%s: %s is on %s, not on %s" % (opname, name, t.device, x.device))
+        if vector:
+            _check_vector(t, name.capitalize(), last)
+        elif tuple(t.shape) != tuple(x.shape):
+            raise InvalidArgumentError(
+                "%s: %s must have the shape %s, got %s"
+                % (opname, name, tuple(x.shape), tuple(t.shape)))
+    return rows, last
+
+
+def MusaAddRmsNorm(x, residual, gamma, epsilon=0.00001, name=None):
+    """The residual's addition with the RMS norm of the last axis behind it, for
+    T in {float, half, bfloat16}: returns (y, sum, inv_rms) with sum = x +
+    residual, inv_rms = rsqrt(mean(sum^2) + epsilon) (fp32, shaped like x with a
+    last axis of 1) and y = sum * inv_rms * gamma.  The norm is that of the
+    unrounded sum; `sum` holds it rounded to T.  One launch where Add and
+    MusaRmsNorm are two with the sum written and read between."""
+    out = _r._native().add_rms_norm(x, residual, gamma, epsilon)
+    if out is not None:
+        return _r._native_result(out, MusaAddRmsNormOutput, "MusaAddRmsNorm")
+    _r._require_cuda()
+    hf = _r._HostForm()
+    xd, rd, g = (hf.to_device(t) for t in (x, residual, gamma))
+    rows, last = _check_rows("MusaAddRmsNorm", xd, [("residual", rd, False), ("gamma", g, True)])
+    xd, rd = xd.contiguous(), rd.contiguous()
+    with torch.cuda.device(xd.device):
+        y, total = torch.empty_like(xd), torch.empty_like(xd)
+        inv = torch.empty(tuple(xd.shape[:-1]) + (1,), dtype=torch.float32, device=xd.device)
+        fn = getattr(_r._lib(), "LaunchAddRmsNorm_" + _r._SUFFIX[xd.dtype])
+        rc = fn(_r._ptr(xd), _r._ptr(rd), _r._ptr(g.contiguous()), _r._ptr(y), _r._ptr(total),
+                _r._ptr(inv), rows, last, float(epsilon), _r._stream())
+        _r._check(rc, "MusaAddRmsNorm")
+    return MusaAddRmsNormOutput(*hf.back_many([y, total, inv]))
+
+
+def MusaAddRmsNormGrad(dy, dsum, sum, inv_rms, gamma, name=None):
+    """The gradient of MusaAddRmsNorm from its stored sum and inv_rms: returns
+    (dx, dgamma).  dx is the gradient of x and of the residual alike; `dsum` is
+    the gradient that reaches `sum` past the norm (None: none does).  dgamma is
+    summed over the rows in a fixed order."""
+    out = _r._native().add_rms_norm_grad(dy, dsum, sum, inv_rms, gamma)
+    if out is not None:
+        return _r._native_result(out, MusaAddRmsNormGradOutput, "MusaAddRmsNormGrad")
+    _r._require_cuda()
+    hf = _r._HostForm()
+    d, ds, s, inv, g = (hf.to_device(t) for t in (dy, dsum, sum, inv_rms, gamma))
+    rows, last = _check_rows("MusaAddRmsNormGrad", s, [
+        ("dy", d, False), ("dsum", ds, False), ("gamma", g, True)])
+    if inv.dtype != torch.float32 or inv.numel() != rows or inv.device != s.device:
+        raise InvalidArgumentError(
+            "MusaAddRmsNormGrad: inv_rms must be float32 with one value per row (%d)" % rows)
+    s, d = s.contiguous(), d.contiguous()
+    ds = None if ds is None else ds.contiguous()
+    with torch.cuda.device(s.device):
+        dx, dgamma = torch.empty_like(s), torch.empty_like(g)
+        if last:
+            lib = _r._lib()
+            ws = _r._scratch(lib.AddRmsNormGradWorkspaceBytes(rows, last), s.device)
+            fn = getattr(lib, "LaunchAddRmsNormGrad_" + _r._SUFFIX[s.dtype])
+            rc = fn(_r._ptr(d), _r._ptr(ds), _r._ptr(s), _r._ptr(inv.contiguous()),
+                    _r._ptr(g.contiguous()), _r._ptr(dx), _r._ptr(dgamma), rows, last,
+                    _r._ptr(ws), ws.numel(), _r._stream())
+            _r._check(rc, "MusaAddRmsNormGrad")
+    return MusaAddRmsNormGradOutput(*hf.back_many([dx, dgamma]))
+
+
+def _quantize(opname, x, residual, gamma, epsilon):
+    out = _r._native().add_rms_norm_quantize(x, residual, gamma, epsilon)
+    if out is not None:
+        return _r._native_result(out, tuple, opname)
+    _r._require_cuda()
+    hf = _r._HostForm()
+    xd, rd, g = (hf.to_device(t) for t in (x, residual, gamma))
+    if hf.kind is not None:
+        raise InvalidArgumentError(
+            "%s: 8-bit outputs have no host form: pass device tensors" % opname)
+    rows, last = _check_rows(opname, xd, [("residual", rd, False), ("gamma", g, True)])
+    xd = xd.contiguous()
+    rd = None if rd is None else rd.contiguous()
+    with torch.cuda.device(xd.device):
+        q = torch.empty(xd.shape, dtype=torch.float8_e4m3fn, device=xd.device)
+        scale = torch.empty(tuple(xd.shape[:-1]) + (1,), dtype=torch.float32, device=xd.device)
+        total = None if rd is None else torch.empty_like(xd)
+        fn = getattr(_r._lib(), "LaunchAddRmsNormQuantize_" + _r._SUFFIX[xd.dtype])
+        rc = fn(_r._ptr(xd), _r._ptr(rd), _r._ptr(None if g is None else g.contiguous()),
+                _r._ptr(q), _r._ptr(scale), _r._ptr(total), rows, last, float(epsilon),
+                _r._stream())
+        _r._check(rc, opname)
+    return q, scale, total
+
+
+def MusaAddRmsNormQuantize(x, residual, gamma, epsilon=0.00001, name=None):
+    """MusaAddRmsNorm with its output in 8 bits: returns (q, scale, sum), q in
+    float8_e4m3fn and scale = max(max|y| / 448, 2^-126) of each row (fp32, shaped
+    like x with a last axis of 1), so that y = q * scale; y itself is not written.
+    `residual` None: the norm of x alone, and sum is None.  A row with a NaN has a
+    NaN scale; rows of length 0 have none."""
+    if gamma is None:
+        raise InvalidArgumentError("MusaAddRmsNormQuantize: gamma is missing")
+    out = _quantize("MusaAddRmsNormQuantize", x, residual, gamma, epsilon)
+    return MusaAddRmsNormQuantizeOutput(*out)
+
+
+def MusaQuantizeRows(x, name=None):
+    """The rows of x (T in {float, half, bfloat16}) in 8 bits: returns (q, scale),
+    x = q * scale, as MusaAddRmsNormQuantize returns them; what lays out the weights
+    [n, k] of MusaQuantizedMatMulBiasAct once."""
+    return MusaQuantizeRowsOutput(*_quantize("MusaQuantizeRows", x, None, None, 0.0)[:2])

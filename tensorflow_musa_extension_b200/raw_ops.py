@@ -33,6 +33,7 @@ except Exception:  # pragma: no cover
     _NP_BF16 = None
 
 ACT_IDENTITY, ACT_RELU, ACT_SWISH, ACT_SIGMOID = 0, 1, 2, 3
+ACT_SILU, ACT_GELU = 4, 5   # matrix products only
 
 logger = logging.getLogger(__name__)
 
@@ -199,6 +200,11 @@ def _workspace(nbytes, device):
         buf = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
         _ws_cache[key] = buf
     return buf
+
+
+def _scratch(nbytes, device):
+    """Scratch of one call, from the caching allocator: a captured graph has its own."""
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
 
 
 def _geometry(shape, data_format):
@@ -852,4 +858,8 @@ from .training_ops import (  # noqa: E402,F401
     MusaResourceApplyGradientDescentMixed, ResourceApplyCenteredRMSProp,
     ResourceApplyGradientDescent, ResourceApplyNadam, ResourceApplyRMSProp)
 from .norm_ops import (  # noqa: E402,F401
-    MusaLayerNorm, MusaLayerNormGrad, MusaRmsNorm, MusaRmsNormGradDx)
+    MusaAddRmsNorm, MusaAddRmsNormGrad, MusaAddRmsNormQuantize, MusaLayerNorm, MusaLayerNormGrad,
+    MusaQuantizeRows, MusaRmsNorm, MusaRmsNormGradDx)
+from .linear_ops import (  # noqa: E402,F401
+    ACTIVATIONS, MusaMatMulBiasAct, MusaMatMulBiasActGrad, MusaQuantizedMatMulBiasAct,
+    check_products)
