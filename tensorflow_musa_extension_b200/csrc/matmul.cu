@@ -18,6 +18,7 @@
 #include "partial_rows.cuh"
 #include "tcgen05_dev.cuh"
 #include "trace.h"
+#include "tuning.h"
 #include "../../include/musa_plugin_kernels.h"
 
 namespace musa_b200 {
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(kSplitThreads)
   }
   __syncwarp();
   if (warp < 4 && last > first) {
-    ok = BarWait(SmemAddr(&done), 0, &give_up, &g_status);
+    ok = __all_sync(0xffffffffu, BarWait(SmemAddr(&done), 0, &give_up, &g_status));
     TmemFenceAfter();
   }
   const int64_t col = col0 + warp * 32 + lane;
@@ -301,6 +302,339 @@ __global__ void __launch_bounds__(kSplitThreads)
     TmemFenceAfter();
     TmemFree<1>(tmem, a.tmem_columns);
   }
+}
+
+// ------------------------------------------------------ products, large sizes --
+
+// A pair of CTAs on two neighbouring SMs computes 256 x tile_n of the product: one matrix
+// instruction covers both (each holds its 128 rows of a and half of b's tile in shared
+// memory, and its 128 rows of the accumulator in tensor memory), so an operand byte is
+// fetched half as often as by two single CTAs.  The pairs are persistent: TMA keeps a ring
+// of five stages (32 KB per CTA) ahead, two accumulators alternate, and eight epilogue
+// warps finish one tile while the next is multiplied.  Their two groups of four take turns
+// of 64 columns: accumulator -> registers -> shared memory (the TMA's swizzled lines) ->
+// one TMA store; the residual comes the same way back.  Outputs that TMA cannot address
+// (odd pitch or base) are moved element by element instead.
+constexpr int kPairStages = 5;
+constexpr int kPairStageBytes = 2 * kSideBytes;
+constexpr int kPairThreads = 384;    // TMA, MMA, tensor memory, idle; 4 .. 11 epilogue
+constexpr int kStagingBytes = 128 * 128;
+constexpr int kPairSmem = kPairStages * kPairStageBytes + 4 * kStagingBytes + 1024;
+constexpr int kBand = 8;             // tile rows walked together, for the L2
+
+struct PairArgs {
+  Epilogue e;
+  int64_t m, n;
+  int blocks;       // stages of depth
+  int tile_n;       // 128 or 256
+  int tiles_m, tiles_n;
+  uint32_t idesc;
+  bool a_rows, b_rows;
+  bool direct;      // y, z and the residual without TMA
+};
+
+// Tile number -> tile row and column: bands of kBand tile rows, columns inside a band.
+__device__ __forceinline__ void TileAt(int tile, const PairArgs& a, int* tm, int* tn) {
+  const int per_band = kBand * a.tiles_n;
+  const int band = tile / per_band, in = tile - band * per_band;
+  const int height = min(kBand, a.tiles_m - band * kBand);
+  *tn = in / height;
+  *tm = band * kBand + in - *tn * height;
+}
+
+__device__ __forceinline__ void GroupBar(int group) {
+  asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+}
+
+// 16-byte piece `piece` of line `line` of a 128-byte-swizzled tile.
+__device__ __forceinline__ uint32_t Swizzled(uint32_t base, int line, int piece) {
+  return base + line * 128 + ((piece ^ (line & 7)) << 4);
+}
+__device__ __forceinline__ uint4 LoadShared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(at)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void StoreShared16(uint32_t at, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y),
+               "r"(v.z), "r"(v.w)
+               : "memory");
+}
+
+// Eight fp32 values to a 16-byte piece.
+template <typename T>
+__device__ __forceinline__ void StorePiece(uint32_t at, const float* v) {
+  Pack<T, 8> p;
+  float2 w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = make_float2(v[2 * i], v[2 * i + 1]);
+  NarrowPack<8>(w, p);
+  StoreShared16(at, *reinterpret_cast<const uint4*>(&p));
+}
+
+// A tile of up to 128 x 64 elements between global memory and swizzled shared memory, by
+// the 128 threads of a group.
+template <typename T, bool kToShared>
+__device__ __forceinline__ void MoveTile(uint32_t tile, T* global, int64_t row0, int64_t col0,
+                                         const PairArgs& a, int thread) {
+  for (int i = thread; i < 128 * 64; i += 128) {
+    const int line = i >> 6, c = i & 63;
+    const uint32_t at = Swizzled(tile, line, c >> 3) + (c & 7) * 2;
+    if (row0 + line < a.m && col0 + c < a.n) {
+      T* g = global + (row0 + line) * a.n + col0 + c;
+      if constexpr (kToShared) {
+        const uint16_t v = *reinterpret_cast<const uint16_t*>(g);
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
+      } else {
+        uint16_t v;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+        *reinterpret_cast<uint16_t*>(g) = v;
+      }
+    }
+  }
+}
+
+template <typename T, bool kBytes>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    PairProductKernel(const __grid_constant__ CUtensorMap a_map,
+                      const __grid_constant__ CUtensorMap b_map,
+                      const __grid_constant__ CUtensorMap y_map,
+                      const __grid_constant__ CUtensorMap z_map,
+                      const __grid_constant__ CUtensorMap r_map,
+                      const __grid_constant__ PairArgs a) {
+  extern __shared__ uint8_t dynamic[];
+  __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2], loaded[2];
+  __shared__ float bias_of[2][64], scale_of[2][64];
+  __shared__ uint32_t tmem_at;
+  __shared__ volatile int give_up;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = static_cast<int>(ClusterCtaRank());
+  const uint32_t ring = (SmemAddr(dynamic) + 1023u) & ~1023u;
+  const uint32_t staging = ring + kPairStages * kPairStageBytes;
+  const int pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+  const int tiles = a.tiles_m * a.tiles_n;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      BarInit(SmemAddr(&full[s]), 1);
+      BarInit(SmemAddr(&empty[s]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      BarInit(SmemAddr(&acc_full[i]), 1);
+      BarInit(SmemAddr(&acc_empty[i]), 16);  // the epilogue warps of both CTAs
+      BarInit(SmemAddr(&loaded[i]), 1);
+    }
+    give_up = 0;
+    BarInitFence();
+  }
+  if (warp == 2) TmemAlloc<2>(SmemAddr(&tmem_at), 512);
+  TmemFenceBefore();
+  __syncthreads();
+  ClusterSync();  // the peer's barriers are initialised
+  TmemFenceAfter();
+  const uint32_t tmem = tmem_at;
+
+  if (warp == 0 && lane == 0) {
+    constexpr int kDepth = kBytes ? kDepthBytes : kDepthBytes / 2;
+    const int half_n = a.tile_n / 2;
+    const uint32_t bytes = 2 * (kSideBytes + half_n * kDepthBytes);
+    int i = 0;
+    bool ok = true;
+    for (int tile = pair; tile < tiles && ok; tile += pairs) {
+      int tm, tn;
+      TileAt(tile, a, &tm, &tn);
+      const int row = tm * 256 + rank * 128, col = tn * a.tile_n + rank * half_n;
+      for (int k = 0; k < a.blocks; ++k, ++i) {
+        const int s = i % kPairStages;
+        ok = BarWait(SmemAddr(&empty[s]), ((i / kPairStages) & 1) ^ 1, &give_up, &g_status);
+        if (!ok) break;
+        const uint32_t at = ring + s * kPairStageBytes;
+        const uint32_t bar = MapToCta(SmemAddr(&full[s]), 0);
+        if (rank == 0) BarExpect(SmemAddr(&full[s]), bytes);
+        const int depth = k * kDepth;
+        if (a.a_rows) {
+          for (int b = 0; b < 2; ++b) {
+            TmaLoad<true>(at + b * kBlockBytes, &a_map, row + b * 64, depth, bar);
+          }
+        } else {
+          TmaLoad<true>(at, &a_map, depth, row, bar);
+        }
+        if (a.b_rows) {
+          for (int b = 0; b < half_n / 64; ++b) {
+            TmaLoad<true>(at + kSideBytes + b * kBlockBytes, &b_map, col + b * 64, depth, bar);
+          }
+        } else {
+          TmaLoad<true>(at + kSideBytes, &b_map, depth, col, bar);
+        }
+      }
+    }
+    // The last arrivals on this CTA's barriers, before it may leave.
+    for (int j = i > kPairStages ? i - kPairStages : 0; j < i && ok; ++j) {
+      ok = BarWait(SmemAddr(&empty[j % kPairStages]), (j / kPairStages) & 1, &give_up, &g_status);
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    const uint32_t a_step = DepthStep(a.a_rows), b_step = DepthStep(a.b_rows);
+    int i = 0, turn = 0;
+    bool ok = true;
+    for (int tile = pair; tile < tiles && ok; tile += pairs, ++turn) {
+      const int buffer = turn & 1;
+      ok = BarWait(SmemAddr(&acc_empty[buffer]), ((turn >> 1) & 1) ^ 1, &give_up, &g_status);
+      if (!ok) break;
+      TmemFenceAfter();
+      const uint32_t acc = tmem + buffer * 256;
+      for (int k = 0; k < a.blocks; ++k, ++i) {
+        const int s = i % kPairStages;
+        ok = BarWait(SmemAddr(&full[s]), (i / kPairStages) & 1, &give_up, &g_status);
+        if (!ok) break;
+        TmemFenceAfter();
+        const uint32_t at = ring + s * kPairStageBytes;
+        const uint64_t ad = OperandDesc(at, a.a_rows);
+        const uint64_t bd = OperandDesc(at + kSideBytes, a.b_rows);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          Mma<2, kBytes>(acc, ad + j * a_step, bd + j * b_step, a.idesc, k > 0 || j > 0);
+        }
+        MmaCommit<2>(SmemAddr(&empty[s]));
+      }
+      if (ok) MmaCommit<2>(SmemAddr(&acc_full[buffer]));
+    }
+  } else if (warp >= 4) {
+    const Epilogue& e = a.e;
+    const int group = (warp - 4) / 4, thread = threadIdx.x - 128 - group * 128;
+    const int line = (warp & 3) * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
+    const bool keep = e.z != nullptr, add = e.residual != nullptr;
+    int turn = 0, slot = 0, loads = 0;
+    bool ok = true;
+    // Threads of a group that gave up a wait go on (without stores): the others count on them
+    // at the group's barriers, and every later wait ends at once.
+    for (int tile = pair; tile < tiles; tile += pairs, ++turn) {
+      int tm, tn;
+      TileAt(tile, a, &tm, &tn);
+      const int buffer = turn & 1;
+      const int64_t row0 = static_cast<int64_t>(tm) * 256 + rank * 128;
+      const float row_scale =
+          kBytes && row0 + line < a.m ? e.a_scale[row0 + line] : 1.0f;
+      for (int c = group; c < a.tile_n / 64; c += 2) {
+        const int64_t col0 = static_cast<int64_t>(tn) * a.tile_n + c * 64;
+        const bool inside = row0 < a.m && col0 < a.n;
+        const uint32_t z_tile = staging + (group * 2 + (slot ^ 1)) * kStagingBytes;
+        const uint32_t y_tile = staging + (group * 2 + slot) * kStagingBytes;
+        if (!keep && inside) slot ^= 1;
+        // The stores that last read these tiles are done with them.
+        if (thread == 0 && !a.direct) {
+          if (keep) TmaStoreWaitRead<0>();
+          else TmaStoreWaitRead<1>();
+          if (add && inside) {
+            BarExpect(SmemAddr(&loaded[group]), kStagingBytes);
+            TmaLoad<false>(y_tile, &r_map, static_cast<int>(col0), static_cast<int>(row0),
+                           SmemAddr(&loaded[group]));
+          }
+        }
+        if (a.direct) {
+          GroupBar(group);
+          if (add && inside) {
+            MoveTile<T, true>(y_tile, const_cast<T*>(static_cast<const T*>(e.residual)), row0,
+                              col0, a, thread);
+          }
+        }
+        if (thread < 64) {
+          const bool there = col0 + thread < a.n;
+          bias_of[group][thread] =
+              there && e.bias != nullptr ? ToF32(static_cast<const T*>(e.bias)[col0 + thread])
+                                         : 0.0f;
+          if (kBytes) scale_of[group][thread] = there ? e.b_scale[col0 + thread] : 1.0f;
+        }
+        GroupBar(group);
+        if (c == group) {
+          ok = BarWait(SmemAddr(&acc_full[buffer]), (turn >> 1) & 1, &give_up, &g_status) && ok;
+          __syncwarp();
+          TmemFenceAfter();
+        }
+        if (add && inside && !a.direct) {
+          ok = BarWait(SmemAddr(&loaded[group]), loads & 1, &give_up, &g_status) && ok;
+          ++loads;
+          __syncwarp();
+        }
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          float v[32];
+          TmemLoad(lanes + buffer * 256 + c * 64 + h * 32, v);
+          TmemLoadWait(v);
+          if (h == 1 && c + 2 >= a.tile_n / 64) {
+            // All of this warp's accumulator is in registers.
+            TmemFenceBefore();
+            __syncwarp();
+            if (lane == 0) BarArriveCluster(MapToCta(SmemAddr(&acc_empty[buffer]), 0));
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(&bias_of[group][h * 32 + i]);
+            if constexpr (kBytes) {
+              const float4 w = *reinterpret_cast<const float4*>(&scale_of[group][h * 32 + i]);
+              v[i] *= row_scale * w.x;
+              v[i + 1] *= row_scale * w.y;
+              v[i + 2] *= row_scale * w.z;
+              v[i + 3] *= row_scale * w.w;
+            }
+            v[i] += b.x;
+            v[i + 1] += b.y;
+            v[i + 2] += b.z;
+            v[i + 3] += b.w;
+          }
+          if (keep) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              StorePiece<T>(Swizzled(z_tile, line, h * 4 + i), v + i * 8);
+            }
+          }
+          Activate(v, e.act);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t at = Swizzled(y_tile, line, h * 4 + i);
+            if (add) {
+              const uint4 w = LoadShared16(at);
+              float2 r[4];
+              WidenPack<8>(*reinterpret_cast<const Pack<T, 8>*>(&w), r);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                v[i * 8 + 2 * q] += r[q].x;
+                v[i * 8 + 2 * q + 1] += r[q].y;
+              }
+            }
+            StorePiece<T>(at, v + i * 8);
+          }
+        }
+        if (a.direct) {
+          GroupBar(group);
+          if (inside) {
+            if (keep) MoveTile<T, false>(z_tile, static_cast<T*>(e.z), row0, col0, a, thread);
+            MoveTile<T, false>(y_tile, static_cast<T*>(e.y), row0, col0, a, thread);
+          }
+        } else {
+          FenceAsyncShared();
+          GroupBar(group);
+          if (thread == 0 && inside && ok) {
+            if (keep) TmaStore(&z_map, static_cast<int>(col0), static_cast<int>(row0), z_tile);
+            TmaStore(&y_map, static_cast<int>(col0), static_cast<int>(row0), y_tile);
+            TmaStoreCommit();
+          }
+        }
+      }
+    }
+    if (thread == 0) TmaStoreWaitAll();
+  }
+  __syncwarp();
+  TmemFenceBefore();
+  __syncthreads();
+  if (give_up != 0) LeaveInFlight();
+  ClusterSync();  // nobody signals or reads a CTA that has left
+  TmemFenceAfter();
+  if (warp == 2) TmemFree<2>(tmem, 512);
 }
 
 // ---------------------------------------------------------------- factors --
@@ -474,8 +808,90 @@ int LaunchSplit(int64_t m, int64_t n, int64_t k, const Factor& fa, const Factor&
 }
 
 template <typename T, bool kBytes>
+int LaunchPair(int64_t m, int64_t n, int64_t k, const Factor& fa, const Factor& fb,
+               const Epilogue& e, int tile_n, cudaStream_t stream) {
+  using E = std::conditional_t<kBytes, uint8_t, T>;
+  constexpr int kDepth = 128 / sizeof(E);
+  PairArgs a = {};
+  a.e = e;
+  a.m = m;
+  a.n = n;
+  a.blocks = static_cast<int>(CeilDiv(k, kDepth));
+  a.tile_n = tile_n;
+  a.tiles_m = static_cast<int>(CeilDiv(m, 256));
+  a.tiles_n = static_cast<int>(CeilDiv(n, tile_n));
+  a.a_rows = fa.rows_contiguous;
+  a.b_rows = fb.rows_contiguous;
+  constexpr int kType = kBytes ? 0 : std::is_same_v<T, __nv_bfloat16> ? 1 : 0;
+  a.idesc = InstructionDesc(kType, a.a_rows, a.b_rows, 256, tile_n);
+  a.direct = n % 8 != 0 || !Aligned16(e.y) || !Aligned16(e.z) || !Aligned16(e.residual);
+  CUtensorMap maps[5] = {};
+  const Lines al = LinesOf(fa, m, k), bl = LinesOf(fb, n, k);
+  bool ok = MakeMap<E>(&maps[0], fa.p, al.count, al.length, fa.ld, a.a_rows ? 64 : 128) &&
+            MakeMap<E>(&maps[1], fb.p, bl.count, bl.length, fb.ld, a.b_rows ? 64 : tile_n / 2);
+  if (!a.direct) {
+    ok = ok && MakeMap<T>(&maps[2], e.y, m, n, n, 128);
+    if (e.z != nullptr) ok = ok && MakeMap<T>(&maps[3], e.z, m, n, n, 128);
+    if (e.residual != nullptr) ok = ok && MakeMap<T>(&maps[4], e.residual, m, n, n, 128);
+  }
+  if (!ok) return MUSA_KERNELS_EINVAL;
+  static std::atomic<int> ready[kMaxDevices];
+  PerDevice(ready, [] {
+    return cudaFuncSetAttribute(PairProductKernel<T, kBytes>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kPairSmem) == cudaSuccess
+               ? 1
+               : 0;
+  });
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(SmCount()));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  // The pairs that run at once (SMs of one processing cluster pair up).
+  static std::atomic<int> resident[kMaxDevices];
+  const int most = PerDevice(resident, [&cfg] {
+    int clusters = 0;
+    cfg.gridDim = dim3(static_cast<unsigned>(SmCount() / 2 * 2));
+    if (cudaOccupancyMaxActiveClusters(&clusters, PairProductKernel<T, kBytes>, &cfg) !=
+            cudaSuccess ||
+        clusters < 1) {
+      cudaGetLastError();
+      clusters = SmCount() / 2;
+    }
+    return clusters;
+  });
+  const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < most ? tiles : most)));
+  CountKernelLaunch();
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, PairProductKernel<T, kBytes>, maps[0], maps[1],
+                                             maps[2], maps[3], maps[4], a));
+}
+
+// Which form: pairs where their tiles come near to filling the machine, columns of 128
+// where those of 256 leave it a third empty; the split form below that.
+template <typename T, bool kBytes>
 int Product(int64_t m, int64_t n, int64_t k, const Factor& fa, const Factor& fb,
             const Epilogue& e, cudaStream_t stream) {
+  const int form = GetTuning(kTuneMatMulForm);
+  int tile_n = 0;
+  if (form == 0) {
+    const int64_t pairs = SmCount() / 2;
+    const int64_t wide = CeilDiv(m, 256) * CeilDiv(n, 256);
+    const int64_t narrow = CeilDiv(m, 256) * CeilDiv(n, 128);
+    if (m > 128 && k > 0 && wide * 3 >= pairs * 2) tile_n = 256;
+    else if (m > 128 && k > 0 && narrow * 3 >= pairs * 2) tile_n = 128;
+  } else if (form >= 2 && k > 0) {
+    tile_n = form == 2 ? 256 : 128;
+  }
+  if (tile_n != 0) return LaunchPair<T, kBytes>(m, n, k, fa, fb, e, tile_n, stream);
   return LaunchSplit<T, kBytes>(m, n, k, fa, fb, e, stream);
 }
 

@@ -41,7 +41,9 @@ enum TuningKey {
   kTuneRowCtas = 27,        // most CTAs per SM of the row kernels; 0: by rule
   kTuneBnGridRefuse = 28,   // 1: the grid-wide form's launch answers that it is too large for the context
                             // (what the caller does then is tested with it)
-  kTuneCount = 29
+  kTuneMatMulForm = 29,     // form of the matrix products: 0 by rule, 1 split, 2 and 3 pairs of CTAs with
+                            // tiles of 256 and 128 columns
+  kTuneCount = 30
 };
 
 int GetTuning(int key);

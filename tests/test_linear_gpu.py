@@ -81,9 +81,18 @@ def _forward(a, b, bias, residual, act, ta, tb, dtype):
     return y, z, y_off + _half(dtype) * (y.abs() + y_off), off + _half(dtype) * (z.abs() + off)
 
 
+@pytest.fixture(params=["by rule", "split", "pairs of 256", "pairs of 128"])
+def form(request, kernel_lib):
+    """Every form of the products on every size."""
+    old = kernel_lib.MusaKernelsSetTuning(29, ["by rule", "split", "pairs of 256",
+                                               "pairs of 128"].index(request.param))
+    yield request.param
+    kernel_lib.MusaKernelsSetTuning(29, old)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("m,n,k", SIZES)
-def test_forward(kernel_lib, dtype, m, n, k):
+def test_forward(form, dtype, m, n, k):
     for i, (ta, tb) in enumerate(((False, False), (False, True), (True, False), (True, True))):
         act = ACTS[(m + n + i) % len(ACTS)]
         a = _rand((k, m) if ta else (m, k), dtype, 1)
@@ -122,7 +131,7 @@ def _backward(dy, a, b, z, act, ta, tb, dtype):
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("m,n,k", SIZES)
-def test_gradient(kernel_lib, dtype, m, n, k):
+def test_gradient(form, dtype, m, n, k):
     for i, (ta, tb) in enumerate(((False, False), (False, True), (True, False), (True, True))):
         act = ACTS[(m + n + i) % len(ACTS)]
         a = _rand((k, m) if ta else (m, k), dtype, 1)
@@ -172,7 +181,7 @@ def _quantized(m, k, seed, std=1.0):
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("m,n,k", SIZES)
-def test_quantized(kernel_lib, dtype, m, n, k):
+def test_quantized(form, dtype, m, n, k):
     act = ACTS[(m + n) % len(ACTS)]
     a, sa = _quantized(m, k, 1)
     b, sb = _quantized(n, k, 2, k ** -0.5)
@@ -188,7 +197,7 @@ def test_quantized(kernel_lib, dtype, m, n, k):
 
 @pytest.mark.parametrize("m,n,k", [(2049, 1300, 700), (700, 5000, 1100), (4100, 520, 2050),
                                    (300, 300, 20000)])
-def test_larger_sizes(kernel_lib, m, n, k):
+def test_larger_sizes(form, m, n, k):
     a, b = _rand((m, k), BF16, 1), _rand((k, n), BF16, 2, k ** -0.5)
     bias, res, dy = _rand((n,), BF16, 3), _rand((m, n), BF16, 4), _rand((m, n), BF16, 5)
     want, wz, tol, tz = _forward(a, b, bias, res, "Gelu", False, False, BF16)
@@ -249,7 +258,7 @@ def _forms(t):
 
 
 @pytest.mark.parametrize("m,n,k", [(5, 48, 72), (300, 264, 520)])
-def test_strides_and_alignment(kernel_lib, m, n, k):
+def test_strides_and_alignment(form, m, n, k):
     a, b = _rand((m, k), BF16, 1), _rand((k, n), BF16, 2, k ** -0.5)
     dy, z = _rand((m, n), BF16, 3), _rand((m, n), BF16, 4)
     bias, res = _rand((n,), BF16, 5), _rand((m, n), BF16, 6)
@@ -273,7 +282,7 @@ def test_strides_and_alignment(kernel_lib, m, n, k):
             assert torch.equal(y, want)
 
 
-def test_values_that_are_not_finite(kernel_lib):
+def test_values_that_are_not_finite(form):
     """They stay in their row or column: no element reads its neighbours' masked lanes."""
     a, b = _rand((20, 30), BF16, 1), _rand((30, 50), BF16, 2)
     want = raw_ops.MusaMatMulBiasAct(a, b)
@@ -291,7 +300,7 @@ def test_values_that_are_not_finite(kernel_lib):
     assert raw_ops.MusaMatMulBiasAct(store[:20, :30], b.nan_to_num(0.0, 0.0, 0.0)).isfinite().all()
 
 
-def test_outputs_stay_inside_their_tensors(kernel_lib):
+def test_outputs_stay_inside_their_tensors(form, kernel_lib):
     """Launchers on a part of a larger buffer: what surrounds it keeps its values."""
     lib = kernel_lib
     for m, n, k in ((3, 5, 7), (130, 257, 64), (300, 600, 128), (600, 1001, 72)):
@@ -324,7 +333,7 @@ def _step_inputs(seed, odd):
 
 
 @pytest.mark.parametrize("odd", [False, True])
-def test_several_threads_and_streams(kernel_lib, odd):
+def test_several_threads_and_streams(form, odd):
     inputs = [_step_inputs(10 * i, odd) for i in range(4)]
     want = [_step(*a) for a in inputs]
     torch.cuda.synchronize()
@@ -352,7 +361,7 @@ def test_several_threads_and_streams(kernel_lib, odd):
 
 @pytest.mark.parametrize("native", [True, False])
 @pytest.mark.parametrize("odd", [False, True])
-def test_graph_capture(monkeypatch, kernel_lib, odd, native):
+def test_graph_capture(monkeypatch, form, odd, native):
     """Two captured graphs replayed at once on streams of their own, on new inputs: the bits
     of the eager calls (each graph has its own scratch)."""
     if not native:
