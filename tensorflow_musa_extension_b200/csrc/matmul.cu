@@ -190,6 +190,8 @@ __global__ void __launch_bounds__(kSplitThreads)
   TmemFenceAfter();
   const uint32_t tmem = tmem_at;
   bool ok = true;
+  GridDepWait();
+  GridDepLaunch();
 
   if (warp == 4 && lane == 0) {
     constexpr int kDepth = kBytes ? kDepthBytes : kDepthBytes / 2;  // elements
@@ -436,6 +438,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   __syncthreads();
   ClusterSync();  // the peer's barriers are initialised
   TmemFenceAfter();
+  GridDepWait();
+  GridDepLaunch();
   const uint32_t tmem = tmem_at;
 
   if (warp == 0 && lane == 0) {
@@ -795,13 +799,15 @@ int LaunchSplit(int64_t m, int64_t n, int64_t k, const Factor& fa, const Factor&
   cfg.blockDim = dim3(kSplitThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = static_cast<unsigned>(a.splits);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = static_cast<unsigned>(a.splits);
   cfg.attrs = attr;
-  cfg.numAttrs = a.splits > 1 ? 1 : 0;
+  cfg.numAttrs = a.splits > 1 ? 2 : 1;
   CountKernelLaunch();
   return static_cast<int>(
       cudaLaunchKernelEx(&cfg, SplitProductKernel<T, kBytes>, p_map, q_map, a));
@@ -848,11 +854,13 @@ int LaunchPair(int64_t m, int64_t n, int64_t k, const Factor& fa, const Factor& 
   cfg.blockDim = dim3(kPairThreads);
   cfg.dynamicSmemBytes = kPairSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   // The pairs that run at once (SMs of one processing cluster pair up).
@@ -870,6 +878,7 @@ int LaunchPair(int64_t m, int64_t n, int64_t k, const Factor& fa, const Factor& 
   });
   const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
   cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < most ? tiles : most)));
+  cfg.numAttrs = 2;
   CountKernelLaunch();
   return static_cast<int>(cudaLaunchKernelEx(&cfg, PairProductKernel<T, kBytes>, maps[0], maps[1],
                                              maps[2], maps[3], maps[4], a));

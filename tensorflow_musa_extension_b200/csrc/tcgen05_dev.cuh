@@ -37,7 +37,7 @@ __device__ __forceinline__ bool BarTry(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
       "{\n.reg .pred p;\n"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
       "selp.u32 %0, 1, 0, p;\n}\n"
       : "=r"(done)
       : "r"(bar), "r"(parity)
