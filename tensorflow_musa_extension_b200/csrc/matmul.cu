@@ -312,15 +312,16 @@ __global__ void __launch_bounds__(kSplitThreads)
 // instruction covers both (each holds its 128 rows of a and half of b's tile in shared
 // memory, and its 128 rows of the accumulator in tensor memory), so an operand byte is
 // fetched half as often as by two single CTAs.  The pairs are persistent: TMA keeps a ring
-// of five stages (32 KB per CTA) ahead, two accumulators alternate, and eight epilogue
-// warps finish one tile while the next is multiplied.  Their two groups of four take turns
-// of 64 columns: accumulator -> registers -> shared memory (the TMA's swizzled lines) ->
-// one TMA store; the residual comes the same way back.  Outputs that TMA cannot address
+// of six stages (32 KB per CTA) ahead, two accumulators alternate, and eight epilogue
+// warps finish one tile while the next is multiplied.  Their two groups of four halve the
+// columns and go 32 at a time: accumulator -> registers -> shared memory (the TMA's
+// swizzled lines of 64 bytes) -> one TMA store; the residual comes the same way back.  Outputs that TMA cannot address
 // (odd pitch or base) are moved element by element instead.
-constexpr int kPairStages = 5;
+constexpr int kPairStages = 6;
 constexpr int kPairStageBytes = 2 * kSideBytes;
 constexpr int kPairThreads = 384;    // TMA, MMA, tensor memory, idle; 4 .. 11 epilogue
-constexpr int kStagingBytes = 128 * 128;
+constexpr int kChunk = 32;           // columns of the epilogue
+constexpr int kStagingBytes = 128 * kChunk * 2;
 constexpr int kPairSmem = kPairStages * kPairStageBytes + 4 * kStagingBytes + 1024;
 constexpr int kBand = 8;             // tile rows walked together, for the L2
 
@@ -348,9 +349,9 @@ __device__ __forceinline__ void GroupBar(int group) {
   asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
 }
 
-// 16-byte piece `piece` of line `line` of a 128-byte-swizzled tile.
+// 16-byte piece `piece` of line `line` of a tile of 64-byte lines with the 64-byte swizzle.
 __device__ __forceinline__ uint32_t Swizzled(uint32_t base, int line, int piece) {
-  return base + line * 128 + ((piece ^ (line & 7)) << 4);
+  return base + line * 64 + ((piece ^ ((line >> 1) & 3)) << 4);
 }
 __device__ __forceinline__ uint4 LoadShared16(uint32_t at) {
   uint4 v;
@@ -377,13 +378,13 @@ __device__ __forceinline__ void StorePiece(uint32_t at, const float* v) {
   StoreShared16(at, *reinterpret_cast<const uint4*>(&p));
 }
 
-// A tile of up to 128 x 64 elements between global memory and swizzled shared memory, by
+// A tile of up to 128 x kChunk elements between global memory and swizzled shared memory, by
 // the 128 threads of a group.
 template <typename T, bool kToShared>
 __device__ __forceinline__ void MoveTile(uint32_t tile, T* global, int64_t row0, int64_t col0,
                                          const PairArgs& a, int thread) {
-  for (int i = thread; i < 128 * 64; i += 128) {
-    const int line = i >> 6, c = i & 63;
+  for (int i = thread; i < 128 * kChunk; i += 128) {
+    const int line = i / kChunk, c = i % kChunk;
     const uint32_t at = Swizzled(tile, line, c >> 3) + (c & 7) * 2;
     if (row0 + line < a.m && col0 + c < a.n) {
       T* g = global + (row0 + line) * a.n + col0 + c;
@@ -409,7 +410,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                       const __grid_constant__ PairArgs a) {
   extern __shared__ uint8_t dynamic[];
   __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2], loaded[2];
-  __shared__ float bias_of[2][64], scale_of[2][64];
+  __shared__ __align__(16) T bias_of[2][128];
+  __shared__ __align__(16) float scale_of[2][kBytes ? 128 : 4];
   __shared__ uint32_t tmem_at;
   __shared__ volatile int give_up;
 
@@ -523,14 +525,34 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int64_t row0 = static_cast<int64_t>(tm) * 256 + rank * 128;
       const float row_scale =
           kBytes && row0 + line < a.m ? e.a_scale[row0 + line] : 1.0f;
-      for (int c = group; c < a.tile_n / 64; c += 2) {
-        const int64_t col0 = static_cast<int64_t>(tn) * a.tile_n + c * 64;
+      const int columns = a.tile_n / 2;
+      const int64_t first = static_cast<int64_t>(tn) * a.tile_n + group * columns;
+      if (thread < columns) {
+        const bool there = first + thread < a.n;
+        bias_of[group][thread] =
+            there && e.bias != nullptr ? static_cast<const T*>(e.bias)[first + thread]
+                                       : FromF32<T>(0.0f);
+        if (kBytes) scale_of[group][thread] = there ? e.b_scale[first + thread] : 1.0f;
+      }
+      ok = BarWait(SmemAddr(&acc_full[buffer]), (turn >> 1) & 1, &give_up, &g_status) && ok;
+      __syncwarp();
+      TmemFenceAfter();
+      for (int c = 0; c < columns; c += kChunk) {
+        const int64_t col0 = first + c;
         const bool inside = row0 < a.m && col0 < a.n;
         const uint32_t z_tile = staging + (group * 2 + (slot ^ 1)) * kStagingBytes;
         const uint32_t y_tile = staging + (group * 2 + slot) * kStagingBytes;
         if (!keep && inside) slot ^= 1;
+        float v[kChunk];
+        TmemLoad(lanes + buffer * 256 + group * columns + c, v);
         // The stores that last read these tiles are done with them.
-        if (thread == 0 && !a.direct) {
+        if (a.direct) {
+          GroupBar(group);
+          if (add && inside) {
+            MoveTile<T, true>(y_tile, const_cast<T*>(static_cast<const T*>(e.residual)), row0,
+                              col0, a, thread);
+          }
+        } else if (thread == 0) {
           if (keep) TmaStoreWaitRead<0>();
           else TmaStoreWaitRead<1>();
           if (add && inside) {
@@ -539,79 +561,56 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                            SmemAddr(&loaded[group]));
           }
         }
-        if (a.direct) {
-          GroupBar(group);
-          if (add && inside) {
-            MoveTile<T, true>(y_tile, const_cast<T*>(static_cast<const T*>(e.residual)), row0,
-                              col0, a, thread);
+        GroupBar(group);
+        TmemLoadWait(v);
+        if (c + kChunk >= columns) {
+          // All of this warp's accumulator is in registers.
+          TmemFenceBefore();
+          __syncwarp();
+          if (lane == 0) BarArriveCluster(MapToCta(SmemAddr(&acc_empty[buffer]), 0));
+        }
+#pragma unroll
+        for (int i = 0; i < kChunk; i += 4) {
+          float2 b[2];
+          WidenPack<4>(*reinterpret_cast<const Pack<T, 4>*>(&bias_of[group][c + i]), b);
+          if constexpr (kBytes) {
+            const float4 w = *reinterpret_cast<const float4*>(&scale_of[group][c + i]);
+            v[i] *= row_scale * w.x;
+            v[i + 1] *= row_scale * w.y;
+            v[i + 2] *= row_scale * w.z;
+            v[i + 3] *= row_scale * w.w;
+          }
+          v[i] += b[0].x;
+          v[i + 1] += b[0].y;
+          v[i + 2] += b[1].x;
+          v[i + 3] += b[1].y;
+        }
+        if (keep) {
+#pragma unroll
+          for (int i = 0; i < kChunk / 8; ++i) {
+            StorePiece<T>(Swizzled(z_tile, line, i), v + i * 8);
           }
         }
-        if (thread < 64) {
-          const bool there = col0 + thread < a.n;
-          bias_of[group][thread] =
-              there && e.bias != nullptr ? ToF32(static_cast<const T*>(e.bias)[col0 + thread])
-                                         : 0.0f;
-          if (kBytes) scale_of[group][thread] = there ? e.b_scale[col0 + thread] : 1.0f;
-        }
-        GroupBar(group);
-        if (c == group) {
-          ok = BarWait(SmemAddr(&acc_full[buffer]), (turn >> 1) & 1, &give_up, &g_status) && ok;
-          __syncwarp();
-          TmemFenceAfter();
-        }
+        Activate(v, e.act);
         if (add && inside && !a.direct) {
           ok = BarWait(SmemAddr(&loaded[group]), loads & 1, &give_up, &g_status) && ok;
           ++loads;
           __syncwarp();
         }
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          float v[32];
-          TmemLoad(lanes + buffer * 256 + c * 64 + h * 32, v);
-          TmemLoadWait(v);
-          if (h == 1 && c + 2 >= a.tile_n / 64) {
-            // All of this warp's accumulator is in registers.
-            TmemFenceBefore();
-            __syncwarp();
-            if (lane == 0) BarArriveCluster(MapToCta(SmemAddr(&acc_empty[buffer]), 0));
-          }
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(&bias_of[group][h * 32 + i]);
-            if constexpr (kBytes) {
-              const float4 w = *reinterpret_cast<const float4*>(&scale_of[group][h * 32 + i]);
-              v[i] *= row_scale * w.x;
-              v[i + 1] *= row_scale * w.y;
-              v[i + 2] *= row_scale * w.z;
-              v[i + 3] *= row_scale * w.w;
-            }
-            v[i] += b.x;
-            v[i + 1] += b.y;
-            v[i + 2] += b.z;
-            v[i + 3] += b.w;
-          }
-          if (keep) {
+        for (int i = 0; i < kChunk / 8; ++i) {
+          const uint32_t at = Swizzled(y_tile, line, i);
+          if (add) {
+            const uint4 w = LoadShared16(at);
+            float2 r[4];
+            WidenPack<8>(*reinterpret_cast<const Pack<T, 8>*>(&w), r);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              StorePiece<T>(Swizzled(z_tile, line, h * 4 + i), v + i * 8);
+            for (int q = 0; q < 4; ++q) {
+              v[i * 8 + 2 * q] += r[q].x;
+              v[i * 8 + 2 * q + 1] += r[q].y;
             }
           }
-          Activate(v, e.act);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t at = Swizzled(y_tile, line, h * 4 + i);
-            if (add) {
-              const uint4 w = LoadShared16(at);
-              float2 r[4];
-              WidenPack<8>(*reinterpret_cast<const Pack<T, 8>*>(&w), r);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                v[i * 8 + 2 * q] += r[q].x;
-                v[i * 8 + 2 * q + 1] += r[q].y;
-              }
-            }
-            StorePiece<T>(at, v + i * 8);
-          }
+          StorePiece<T>(at, v + i * 8);
         }
         if (a.direct) {
           GroupBar(group);
@@ -629,6 +628,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
         }
       }
+      GroupBar(group);  // before the next tile's bias
     }
     if (thread == 0) TmaStoreWaitAll();
   }
@@ -721,7 +721,8 @@ EncodeFn Encode() {
   return fn;
 }
 
-// A map over lines of memory with boxes of 128 bytes x `box_lines`, swizzled.
+// A map over lines of memory with boxes of 128 (or 64) bytes x `box_lines`, swizzled over
+// their width.
 template <typename T>
 constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_UINT8;
 template <>
@@ -731,17 +732,18 @@ constexpr CUtensorMapDataType kMapType<__nv_bfloat16> = CU_TENSOR_MAP_DATA_TYPE_
 
 template <typename E>
 bool MakeMap(CUtensorMap* map, const void* p, int64_t count, int64_t length, int64_t ld,
-             int box_lines) {
+             int box_lines, int box_bytes = 128) {
   const EncodeFn encode = Encode();
   if (encode == nullptr) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(length), static_cast<cuuint64_t>(count)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(
       count > 1 ? ld * static_cast<int64_t>(sizeof(E)) : RoundUp(length * sizeof(E), 16))};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / sizeof(E)),
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_bytes / sizeof(E)),
                              static_cast<cuuint32_t>(box_lines)};
   const cuuint32_t steps[2] = {1, 1};
   return encode(map, kMapType<E>, 2, const_cast<void*>(p), dims, strides, box, steps,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_INTERLEAVE_NONE,
+                box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -836,9 +838,9 @@ int LaunchPair(int64_t m, int64_t n, int64_t k, const Factor& fa, const Factor& 
   bool ok = MakeMap<E>(&maps[0], fa.p, al.count, al.length, fa.ld, a.a_rows ? 64 : 128) &&
             MakeMap<E>(&maps[1], fb.p, bl.count, bl.length, fb.ld, a.b_rows ? 64 : tile_n / 2);
   if (!a.direct) {
-    ok = ok && MakeMap<T>(&maps[2], e.y, m, n, n, 128);
-    if (e.z != nullptr) ok = ok && MakeMap<T>(&maps[3], e.z, m, n, n, 128);
-    if (e.residual != nullptr) ok = ok && MakeMap<T>(&maps[4], e.residual, m, n, n, 128);
+    ok = ok && MakeMap<T>(&maps[2], e.y, m, n, n, 128, 2 * kChunk);
+    if (e.z != nullptr) ok = ok && MakeMap<T>(&maps[3], e.z, m, n, n, 128, 2 * kChunk);
+    if (e.residual != nullptr) ok = ok && MakeMap<T>(&maps[4], e.residual, m, n, n, 128, 2 * kChunk);
   }
   if (!ok) return MUSA_KERNELS_EINVAL;
   static std::atomic<int> ready[kMaxDevices];
