@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kSplitThreads)
   __shared__ uint32_t tmem_at;
   __shared__ volatile int give_up;
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const uint32_t ring = (SmemAddr(dynamic) + 1023u) & ~1023u;
   const uint32_t rank = a.splits > 1 ? ClusterCtaRank() : 0;
   const int64_t col0 = static_cast<int64_t>(blockIdx.x) * 128;
@@ -193,55 +193,66 @@ __global__ void __launch_bounds__(kSplitThreads)
   GridDepWait();
   GridDepLaunch();
 
-  if (warp == 4 && lane == 0) {
+  if (warp == 4) {
     constexpr int kDepth = kBytes ? kDepthBytes : kDepthBytes / 2;  // elements
-    for (int i = 0; i < last - first; ++i) {
-      const int s = i % a.stages;
-      if (!BarWait(SmemAddr(&empty[s]), ((i / a.stages) & 1) ^ 1, &give_up, &g_status)) {
-        ok = false;
-        break;
-      }
+    int s = 0, phase = 1;
+    for (int i = first; i < last; ++i) {
+      if (!BarWait(SmemAddr(&empty[s]), phase, &give_up, &g_status)) break;
       const uint32_t bar = SmemAddr(&full[s]);
       const uint32_t p = ring + s * a.stage_bytes, q = p + kSideBytes;
-      const int depth = (first + i) * kDepth;
-      BarExpect(bar, a.stage_bytes);
-      if (a.p_rows) {
-        for (int b = 0; b < 2; ++b) {
-          TmaLoad<false>(p + b * kBlockBytes, &p_map, static_cast<int>(col0) + b * 64, depth, bar);
+      const int depth = i * kDepth;
+      if (ElectLane()) {
+        BarExpect(bar, a.stage_bytes);
+        if (a.p_rows) {
+          for (int b = 0; b < 2; ++b) {
+            TmaLoad<false>(p + b * kBlockBytes, &p_map, static_cast<int>(col0) + b * 64, depth,
+                           bar);
+          }
+        } else {
+          TmaLoad<false>(p, &p_map, depth, static_cast<int>(col0), bar);
         }
-      } else {
-        TmaLoad<false>(p, &p_map, depth, static_cast<int>(col0), bar);
+        if (a.q_rows) {
+          for (int b = 0; b < a.rows_tile / 64; ++b) {
+            TmaLoad<false>(q + b * kBlockBytes, &q_map, static_cast<int>(row0) + b * 64, depth,
+                           bar);
+          }
+        } else {
+          TmaLoad<false>(q, &q_map, depth, static_cast<int>(row0), bar);
+        }
       }
-      if (a.q_rows) {
-        for (int b = 0; b < a.rows_tile / 64; ++b) {
-          TmaLoad<false>(q + b * kBlockBytes, &q_map, static_cast<int>(row0) + b * 64, depth, bar);
-        }
-      } else {
-        TmaLoad<false>(q, &q_map, depth, static_cast<int>(row0), bar);
+      __syncwarp();
+      if (++s == a.stages) {
+        s = 0;
+        phase ^= 1;
       }
     }
-  } else if (warp == 5 && lane == 0) {
+  } else if (warp == 5 && last > first) {
     const uint32_t p_step = DepthStep(a.p_rows), q_step = DepthStep(a.q_rows);
-    for (int i = 0; i < last - first; ++i) {
-      const int s = i % a.stages;
-      if (!BarWait(SmemAddr(&full[s]), (i / a.stages) & 1, &give_up, &g_status)) {
-        ok = false;
-        break;
-      }
+    int s = 0, phase = 0;
+    for (int i = first; i < last; ++i) {
+      ok = BarWait(SmemAddr(&full[s]), phase, &give_up, &g_status);
+      if (!ok) break;
       TmemFenceAfter();
       const uint32_t p = ring + s * a.stage_bytes;
       const uint64_t pd = OperandDesc(p, a.p_rows), qd = OperandDesc(p + kSideBytes, a.q_rows);
+      if (ElectLane()) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        Mma<1, kBytes>(tmem, pd + j * p_step, qd + j * q_step, a.idesc, i > 0 || j > 0);
+        for (int j = 0; j < 4; ++j) {
+          Mma<1, kBytes>(tmem, pd + j * p_step, qd + j * q_step, a.idesc, i > first || j > 0);
+        }
+        MmaCommit<1>(SmemAddr(&empty[s]));
       }
-      MmaCommit<1>(SmemAddr(&empty[s]));
+      __syncwarp();
+      if (++s == a.stages) {
+        s = 0;
+        phase ^= 1;
+      }
     }
-    if (ok && last > first) MmaCommit<1>(SmemAddr(&done));
+    if (ok && ElectLane()) MmaCommit<1>(SmemAddr(&done));
   }
   __syncwarp();
   if (warp < 4 && last > first) {
-    ok = __all_sync(0xffffffffu, BarWait(SmemAddr(&done), 0, &give_up, &g_status));
+    ok = BarWait(SmemAddr(&done), 0, &give_up, &g_status);
     TmemFenceAfter();
   }
   const int64_t col = col0 + warp * 32 + lane;
@@ -415,7 +426,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   __shared__ uint32_t tmem_at;
   __shared__ volatile int give_up;
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int rank = static_cast<int>(ClusterCtaRank());
   const uint32_t ring = (SmemAddr(dynamic) + 1023u) & ~1023u;
   const uint32_t staging = ring + kPairStages * kPairStageBytes;
@@ -444,47 +455,57 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   GridDepLaunch();
   const uint32_t tmem = tmem_at;
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     constexpr int kDepth = kBytes ? kDepthBytes : kDepthBytes / 2;
     const int half_n = a.tile_n / 2;
     const uint32_t bytes = 2 * (kSideBytes + half_n * kDepthBytes);
-    int i = 0;
+    int s = 0, phase = 1, used = 0;
     bool ok = true;
     for (int tile = pair; tile < tiles && ok; tile += pairs) {
       int tm, tn;
       TileAt(tile, a, &tm, &tn);
       const int row = tm * 256 + rank * 128, col = tn * a.tile_n + rank * half_n;
-      for (int k = 0; k < a.blocks; ++k, ++i) {
-        const int s = i % kPairStages;
-        ok = BarWait(SmemAddr(&empty[s]), ((i / kPairStages) & 1) ^ 1, &give_up, &g_status);
+      for (int k = 0; k < a.blocks; ++k) {
+        ok = BarWait(SmemAddr(&empty[s]), phase, &give_up, &g_status);
         if (!ok) break;
         const uint32_t at = ring + s * kPairStageBytes;
         const uint32_t bar = MapToCta(SmemAddr(&full[s]), 0);
-        if (rank == 0) BarExpect(SmemAddr(&full[s]), bytes);
         const int depth = k * kDepth;
-        if (a.a_rows) {
-          for (int b = 0; b < 2; ++b) {
-            TmaLoad<true>(at + b * kBlockBytes, &a_map, row + b * 64, depth, bar);
+        if (ElectLane()) {
+          if (rank == 0) BarExpect(SmemAddr(&full[s]), bytes);
+          if (a.a_rows) {
+            for (int b = 0; b < 2; ++b) {
+              TmaLoad<true>(at + b * kBlockBytes, &a_map, row + b * 64, depth, bar);
+            }
+          } else {
+            TmaLoad<true>(at, &a_map, depth, row, bar);
           }
-        } else {
-          TmaLoad<true>(at, &a_map, depth, row, bar);
+          if (a.b_rows) {
+            for (int b = 0; b < half_n / 64; ++b) {
+              TmaLoad<true>(at + kSideBytes + b * kBlockBytes, &b_map, col + b * 64, depth, bar);
+            }
+          } else {
+            TmaLoad<true>(at + kSideBytes, &b_map, depth, col, bar);
+          }
         }
-        if (a.b_rows) {
-          for (int b = 0; b < half_n / 64; ++b) {
-            TmaLoad<true>(at + kSideBytes + b * kBlockBytes, &b_map, col + b * 64, depth, bar);
-          }
-        } else {
-          TmaLoad<true>(at + kSideBytes, &b_map, depth, col, bar);
+        __syncwarp();
+        used = min(used + 1, kPairStages);
+        if (++s == kPairStages) {
+          s = 0;
+          phase ^= 1;
         }
       }
     }
     // The last arrivals on this CTA's barriers, before it may leave.
-    for (int j = i > kPairStages ? i - kPairStages : 0; j < i && ok; ++j) {
-      ok = BarWait(SmemAddr(&empty[j % kPairStages]), (j / kPairStages) & 1, &give_up, &g_status);
+    for (int i = 0; i < used && ok; ++i) {
+      // The oldest of them first: stage s, or stage 0 where the ring was not filled.
+      const int at = used == kPairStages ? (s + i) % kPairStages : i;
+      const int turn = used == kPairStages && at >= s ? phase : phase ^ 1;
+      ok = BarWait(SmemAddr(&empty[at]), turn, &give_up, &g_status);
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 1 && rank == 0) {
     const uint32_t a_step = DepthStep(a.a_rows), b_step = DepthStep(a.b_rows);
-    int i = 0, turn = 0;
+    int s = 0, phase = 0, turn = 0;
     bool ok = true;
     for (int tile = pair; tile < tiles && ok; tile += pairs, ++turn) {
       const int buffer = turn & 1;
@@ -492,21 +513,27 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       if (!ok) break;
       TmemFenceAfter();
       const uint32_t acc = tmem + buffer * 256;
-      for (int k = 0; k < a.blocks; ++k, ++i) {
-        const int s = i % kPairStages;
-        ok = BarWait(SmemAddr(&full[s]), (i / kPairStages) & 1, &give_up, &g_status);
+      for (int k = 0; k < a.blocks; ++k) {
+        ok = BarWait(SmemAddr(&full[s]), phase, &give_up, &g_status);
         if (!ok) break;
         TmemFenceAfter();
         const uint32_t at = ring + s * kPairStageBytes;
         const uint64_t ad = OperandDesc(at, a.a_rows);
         const uint64_t bd = OperandDesc(at + kSideBytes, a.b_rows);
+        if (ElectLane()) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          Mma<2, kBytes>(acc, ad + j * a_step, bd + j * b_step, a.idesc, k > 0 || j > 0);
+          for (int j = 0; j < 4; ++j) {
+            Mma<2, kBytes>(acc, ad + j * a_step, bd + j * b_step, a.idesc, k > 0 || j > 0);
+          }
+          MmaCommit<2>(SmemAddr(&empty[s]));
+          if (k == a.blocks - 1) MmaCommit<2>(SmemAddr(&acc_full[buffer]));
         }
-        MmaCommit<2>(SmemAddr(&empty[s]));
+        __syncwarp();
+        if (++s == kPairStages) {
+          s = 0;
+          phase ^= 1;
+        }
       }
-      if (ok) MmaCommit<2>(SmemAddr(&acc_full[buffer]));
     }
   } else if (warp >= 4) {
     const Epilogue& e = a.e;

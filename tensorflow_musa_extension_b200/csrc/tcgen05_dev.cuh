@@ -51,22 +51,35 @@ __device__ __forceinline__ bool BarTry(uint32_t bar, uint32_t parity) {
 // instructions already issued land before the CTA frees what they write.
 constexpr long long kWaitCycles = 4000000000LL;
 
+// A whole warp waits, with one answer for it: the loops around the waits stay uniform, so that
+// their addresses and descriptors live in the uniform registers that the TMA and matrix
+// instructions read (with one lane looping alone a stage took 650 cycles, whatever the tile).
 __device__ __noinline__ bool BarWaitSlow(uint32_t bar, uint32_t parity, volatile int* give_up,
                                          int* status) {
   const long long begin = clock64();
-  while (!BarTry(bar, parity)) {
-    if (*give_up != 0) return false;
-    if (clock64() - begin > kWaitCycles) {
-      *give_up = 1;
-      atomicExch(status, 1);
+  for (;;) {
+    const bool late = clock64() - begin > kWaitCycles;
+    if (__all_sync(0xffffffffu, BarTry(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, late || *give_up != 0)) {
+      if (late) {
+        *give_up = 1;
+        atomicExch(status, 1);
+      }
       return false;
     }
   }
-  return true;
 }
 __device__ __forceinline__ bool BarWait(uint32_t bar, uint32_t parity, volatile int* give_up,
                                         int* status) {
-  return BarTry(bar, parity) || BarWaitSlow(bar, parity, give_up, status);
+  if (__all_sync(0xffffffffu, BarTry(bar, parity))) return true;
+  return __all_sync(0xffffffffu, BarWaitSlow(bar, parity, give_up, status));
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool ElectLane() {
+  uint32_t yes;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(yes));
+  return yes != 0;
 }
 __device__ __forceinline__ void LeaveInFlight() {
   for (int i = 0; i < 2000; ++i) __nanosleep(1000);
