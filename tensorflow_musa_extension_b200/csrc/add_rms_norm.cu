@@ -36,29 +36,36 @@ struct AddNormArgs {
   int row_size;
   int group;             // threads of a row, a power of two
   float epsilon;
+  float inv_size;        // 1 / row_size
 };
 
-// Sum of `v` and largest of `w` over the group's threads (power of two, aligned runs).
+// Sum of `v` and (kMax) largest of `w` over the group's threads (power of two, aligned runs).
+template <bool kMax>
 __device__ __forceinline__ void GroupSumMax(float& v, unsigned& w, int group, float* sums,
                                             unsigned* tops) {
-  const int span = group < 32 ? group : 32;
-  for (int m = span / 2; m > 0; m >>= 1) {
-    v += __shfl_xor_sync(0xffffffffu, v, m);
-    w = max(w, __shfl_xor_sync(0xffffffffu, w, m));
+  if (group >= 32) {
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    if (kMax) w = __reduce_max_sync(0xffffffffu, w);
+  } else {
+    for (int m = group / 2; m > 0; m >>= 1) {
+      v += __shfl_xor_sync(0xffffffffu, v, m);
+      if (kMax) w = max(w, __shfl_xor_sync(0xffffffffu, w, m));
+    }
   }
   if (group > 32) {
     const int warp = threadIdx.x >> 5, warps = group >> 5;
     const int first = warp & ~(warps - 1);
     if ((threadIdx.x & 31) == 0) {
       sums[warp] = v;
-      tops[warp] = w;
+      if (kMax) tops[warp] = w;
     }
     __syncthreads();
     v = 0.0f;
     w = 0;
     for (int i = 0; i < warps; ++i) {
       v += sums[first + i];
-      w = max(w, tops[first + i]);
+      if (kMax) w = max(w, tops[first + i]);
     }
   }
 }
@@ -92,6 +99,28 @@ __device__ __forceinline__ Pack<uint8_t, kVec> ToE4m3(const float (&v)[kVec]) {
   return out;
 }
 
+// Per-thread asynchronous copies of 16 bytes, or of a pack's first `bytes` with zeros behind.
+// A thread reads back only slots that it filled itself.
+__device__ __forceinline__ void CopyPack(uint4* slot, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   static_cast<unsigned>(__cvta_generic_to_shared(slot))),
+               "l"(from)
+               : "memory");
+}
+__device__ __forceinline__ void CopyPart(uint4* slot, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                   static_cast<unsigned>(__cvta_generic_to_shared(slot))),
+               "l"(from), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void CopyCommit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int kPending>
+__device__ __forceinline__ void CopyWait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
 // A row's packs against the tensor: whole packs, or (kShifted) rows of any length, whose
 // first and last pack may hold elements of the neighbouring rows.
 template <typename T, bool kShifted>
@@ -116,15 +145,16 @@ struct RowView {
   __device__ bool Inside(int p, int e) const {
     return static_cast<unsigned>(p * kVec + e - shift) < static_cast<unsigned>(row_size);
   }
-  __device__ Pack<T, kVec> Load(const void* base, int p) const {
+  // Starts the copy of pack p to a slot of shared memory; what lies behind the tensor is
+  // not read and comes as zeros.
+  __device__ void Copy(uint4* slot, const void* base, int p) const {
     const T* at = static_cast<const T*>(base) + first + p * kVec;
-    if (kShifted && first + (p + 1) * static_cast<int64_t>(kVec) > total) {
-      Pack<T, kVec> v;
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) v.v[e] = Inside(p, e) ? at[e] : FromF32<T>(0.0f);
-      return v;
+    const int64_t left = total - (first + static_cast<int64_t>(p) * kVec);
+    if (kShifted && left < kVec) {
+      CopyPart(slot, at, static_cast<int>(left * sizeof(T)));
+    } else {
+      CopyPack(slot, at);
     }
-    return LoadStream(reinterpret_cast<const Pack<T, kVec>*>(at));
   }
   template <typename U>
   __device__ void Store(void* base, int p, const Pack<U, kVec>& v) const {
@@ -152,82 +182,133 @@ struct RowView {
   }
 };
 
+// A CTA of 256 to 1024 threads holds blockDim / group rows and goes round the tensor.  The
+// rows come through a ring of slots in shared memory that asynchronous copies fill: once a
+// thread has added its packs of a row into registers it asks for those of the row kStages
+// rounds on, so the copies run through the reduction and the stores.  A thread meets the
+// same columns in each of its rows (shifted rows: they are a multiple of the pack width
+// apart, the launch sees to it) and keeps their gamma in registers.
+__host__ __device__ constexpr int ForwardStages(int packs) { return packs == 4 ? 1 : 3; }
+
 template <typename T, int kPacks, bool kQuantize, bool kShifted>
 __global__ void __launch_bounds__(1024) AddNormKernel(AddNormArgs a) {
   constexpr int kVec = VecWidth<T>::value;
+  constexpr int kStages = ForwardStages(kPacks);
   using P = Pack<T, kVec>;
-  __shared__ float sums[32];
-  __shared__ unsigned tops[32];
+  __shared__ float sums[2][32];
+  __shared__ unsigned tops[2][32];
+  extern __shared__ uint4 ring[];  // [stage][input][pack][thread]
+  GridDepWait();
+  GridDepLaunch();
   const int t = threadIdx.x & (a.group - 1);
-  const int64_t row =
-      static_cast<int64_t>(blockIdx.x) * (blockDim.x / a.group) + threadIdx.x / a.group;
-  const bool there = row < a.rows;
-  const RowView<T, kShifted> view(there ? row : 0, a.rows, a.row_size);
-  P x[kPacks], r[kPacks], gamma[kPacks];
-  float s[kPacks][kVec];
+  const int lanes = blockDim.x / a.group;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * lanes;
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * lanes;
+  const bool add = !kQuantize || a.residual != nullptr;
+  const bool normed = !kQuantize || a.gamma != nullptr;
+  int64_t row = base + threadIdx.x / a.group;
+  RowView<T, kShifted> view(row, a.rows, a.row_size);
+  const int64_t jump = step * a.row_size;
+  const auto Slot = [&](int stage, int input, int j) {
+    return ring + ((stage * 2 + input) * kPacks + j) * blockDim.x + threadIdx.x;
+  };
+  // Packs of the row `ahead` rounds on to a stage; one group of copies, maybe empty.
+  const auto Ask = [&](int stage, int ahead) {
+    if (row + ahead * step < a.rows) {
+      RowView<T, kShifted> at = view;
+      at.first += ahead * jump;
 #pragma unroll
-  for (int j = 0; j < kPacks; ++j) {
-    const int p = t + j * a.group;
-    if (there && p < view.packs) {
-      x[j] = view.Load(a.x, p);
-      if (!kQuantize || a.residual != nullptr) r[j] = view.Load(a.residual, p);
-      if (!kQuantize || a.gamma != nullptr) gamma[j] = view.Vector(a.gamma, p);
-    }
-  }
-  float square = 0.0f;
-  unsigned top = 0;
-#pragma unroll
-  for (int j = 0; j < kPacks; ++j) {
-    const int p = t + j * a.group;
-    if (there && p < view.packs) {
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        s[j][e] = ToF32(x[j].v[e]);
-        if (!kQuantize || a.residual != nullptr) s[j][e] += ToF32(r[j].v[e]);
-        if (view.Edge(p) && !view.Inside(p, e)) s[j][e] = 0.0f;
-        square = fmaf(s[j][e], s[j][e], square);
-        if constexpr (kQuantize) {
-          const float g = a.gamma != nullptr ? ToF32(gamma[j].v[e]) : 1.0f;
-          top = max(top, MagnitudeBits(s[j][e] * g));
+      for (int j = 0; j < kPacks; ++j) {
+        const int p = t + j * a.group;
+        if (p < view.packs) {
+          at.Copy(Slot(stage, 0, j), a.x, p);
+          if (add) at.Copy(Slot(stage, 1, j), a.residual, p);
         }
       }
     }
-  }
-  GroupSumMax(square, top, a.group, sums, tops);
-  float inv = rsqrtf(square / a.row_size + a.epsilon);
-  if (kQuantize && a.gamma == nullptr) inv = 1.0f;
-  float scale = 1.0f, unscale = 1.0f;
-  if constexpr (kQuantize) {
-    scale = QuantizeScale(__uint_as_float(top) * inv);
-    unscale = 1.0f / scale;
-    if (there && t == 0) a.stat[row] = scale;
-  } else {
-    if (there && t == 0) a.stat[row] = inv;
-  }
+    CopyCommit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) Ask(i, i);
+  P gamma[kPacks];
 #pragma unroll
   for (int j = 0; j < kPacks; ++j) {
     const int p = t + j * a.group;
-    if (there && p < view.packs) {
-      P total;
-      float y[kVec];
+    if (normed && p < view.packs) gamma[j] = view.Vector(a.gamma, p);
+  }
+  // Whole CTAs go round: the reductions of wide groups are barriers.
+  int stage = 0, parity = 0;
+  for (int64_t at = base; at < a.rows; at += step) {
+    const bool there = row < a.rows;
+    CopyWait<kStages - 1>();
+    float s[kPacks][kVec];
+    float square = 0.0f;
+    unsigned top = 0;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        total.v[e] = FromF32<T>(s[j][e]);
-        const float g = !kQuantize || a.gamma != nullptr ? ToF32(gamma[j].v[e]) : 1.0f;
-        y[e] = s[j][e] * inv * g;
-      }
-      if (!kQuantize || a.sum != nullptr) view.Store(a.sum, p, total);
-      if constexpr (kQuantize) {
+    for (int j = 0; j < kPacks; ++j) {
+      const int p = t + j * a.group;
+      if (there && p < view.packs) {
+        const uint4 xw = *Slot(stage, 0, j);
+        float2 x[kVec / 2];
+        WidenPack<kVec>(*reinterpret_cast<const P*>(&xw), x);
+        if (add) {
+          const uint4 rw = *Slot(stage, 1, j);
+          float2 r[kVec / 2];
+          WidenPack<kVec>(*reinterpret_cast<const P*>(&rw), r);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) y[e] = Quotient(y[e], scale, unscale, a.gamma != nullptr);
-        view.Store(a.y, p, ToE4m3<kVec>(y));
-      } else {
-        P out;
+          for (int e = 0; e < kVec / 2; ++e) x[e] = Add2(x[e], r[e]);
+        }
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) out.v[e] = FromF32<T>(y[e]);
-        view.Store(a.y, p, out);
+        for (int e = 0; e < kVec; ++e) {
+          s[j][e] = e % 2 == 0 ? x[e / 2].x : x[e / 2].y;
+          if (view.Edge(p) && !view.Inside(p, e)) s[j][e] = 0.0f;
+          square = fmaf(s[j][e], s[j][e], square);
+          if constexpr (kQuantize) {
+            const float g = normed ? ToF32(gamma[j].v[e]) : 1.0f;
+            top = max(top, MagnitudeBits(s[j][e] * g));
+          }
+        }
       }
     }
+    Ask(stage, kStages);
+    if (++stage == kStages) stage = 0;
+    GroupSumMax<kQuantize>(square, top, a.group, sums[parity], tops[parity]);
+    parity ^= 1;
+    float inv = rsqrtf(fmaf(square, a.inv_size, a.epsilon));
+    if (!normed) inv = 1.0f;
+    float scale = 1.0f, unscale = 1.0f;
+    if constexpr (kQuantize) {
+      scale = QuantizeScale(__uint_as_float(top) * inv);
+      unscale = 1.0f / scale;
+    }
+    if (there && t == 0) a.stat[row] = kQuantize ? scale : inv;
+#pragma unroll
+    for (int j = 0; j < kPacks; ++j) {
+      const int p = t + j * a.group;
+      if (there && p < view.packs) {
+        P total;
+        float y[kVec];
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          total.v[e] = FromF32<T>(s[j][e]);
+          y[e] = s[j][e] * inv;
+          if (normed) y[e] *= ToF32(gamma[j].v[e]);
+        }
+        if (!kQuantize || a.sum != nullptr) view.Store(a.sum, p, total);
+        if constexpr (kQuantize) {
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) y[e] = Quotient(y[e], scale, unscale, normed);
+          view.Store(a.y, p, ToE4m3<kVec>(y));
+        } else {
+          P out;
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) out.v[e] = FromF32<T>(y[e]);
+          view.Store(a.y, p, out);
+        }
+      }
+    }
+    view.first += jump;
+    row += step;
   }
 }
 
@@ -238,6 +319,8 @@ template <typename T, bool kQuantize>
 __global__ void __launch_bounds__(kLoopThreads) AddNormLoopKernel(AddNormArgs a) {
   __shared__ float sums[32];
   __shared__ unsigned tops[32];
+  GridDepWait();
+  GridDepLaunch();
   const T* gamma = static_cast<const T*>(a.gamma);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.row_size;
@@ -251,9 +334,9 @@ __global__ void __launch_bounds__(kLoopThreads) AddNormLoopKernel(AddNormArgs a)
       square = fmaf(s, s, square);
       if (kQuantize) top = max(top, MagnitudeBits(gamma != nullptr ? s * ToF32(gamma[c]) : s));
     }
-    GroupSumMax(square, top, kLoopThreads, sums, tops);
+    GroupSumMax<kQuantize>(square, top, kLoopThreads, sums, tops);
     __syncthreads();  // before the next row's sums
-    float inv = rsqrtf(square / a.row_size + a.epsilon);
+    float inv = rsqrtf(fmaf(square, a.inv_size, a.epsilon));
     if (kQuantize && gamma == nullptr) inv = 1.0f;
     const float scale = kQuantize ? QuantizeScale(__uint_as_float(top) * inv) : 1.0f;
     const float unscale = 1.0f / scale;
@@ -287,91 +370,127 @@ struct AddNormGradArgs {
   int64_t rows;
   int row_size;
   int group;
+  float inv_size;
 };
 
-// A thread meets the same columns in each of its rows (shifted rows: they are a multiple
-// of the pack width apart, the launch sees to it) and keeps their dgamma in registers.  At
-// the end the row lanes of the CTA are added in order and the CTA leaves one partial row.
-constexpr int kGradThreads = 512;
+// As the forward, with the dgamma of a thread's columns in registers too; a row's slots are
+// read twice, before and after its reduction, and asked for again behind its stores.  At the
+// end the row lanes of the CTA are added in order and the CTA leaves one partial row.
+__host__ __device__ constexpr int GradStages(int packs, int threads) {
+  return packs == 4 ? 1 : threads == 1024 ? 2 : 3;
+}
+// CTAs per SM at the registers of 85 and the shared memory of three stages.
+__host__ __device__ constexpr int GradCtas(int threads) { return threads == 1024 ? 1 : 3; }
 
-template <typename T, int kPacks, bool kShifted>
-__global__ void __launch_bounds__(kGradThreads) AddNormGradKernel(AddNormGradArgs a) {
+template <typename T, int kPacks, int kThreads, bool kShifted>
+__global__ void __launch_bounds__(kThreads, GradCtas(kThreads)) AddNormGradKernel(
+    AddNormGradArgs a) {
   constexpr int kVec = VecWidth<T>::value;
+  constexpr int kStages = GradStages(kPacks, kThreads);
   using P = Pack<T, kVec>;
   __shared__ float sums[2][32];
-  __shared__ unsigned tops[2][32];
-  extern __shared__ float columns[];
+  extern __shared__ uint4 ring[];  // [stage][input][pack][thread]
+  GridDepWait();
+  GridDepLaunch();
   const int t = threadIdx.x & (a.group - 1);
   const int lane_row = threadIdx.x / a.group, lanes = blockDim.x / a.group;
-  float acc[kPacks][kVec];
-#pragma unroll
-  for (int j = 0; j < kPacks; ++j) {
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) acc[j][e] = 0.0f;
-  }
+  const int64_t step = static_cast<int64_t>(gridDim.x) * lanes;
+  const int64_t jump = step * a.row_size;
   const int64_t first_row = static_cast<int64_t>(blockIdx.x) * lanes + lane_row;
-  int parity = 0;
-  // Whole CTAs go round: the reductions of wide groups are barriers.
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * lanes; base < a.rows;
-       base += static_cast<int64_t>(gridDim.x) * lanes) {
-    const int64_t row = base + lane_row;
-    const bool there = row < a.rows;
-    const RowView<T, kShifted> view(there ? row : 0, a.rows, a.row_size);
-    P s[kPacks], dy[kPacks], ds[kPacks];
-    float inv = 0.0f;
-    if (there) {
-      inv = a.inv[row];
+  int64_t row = first_row;
+  RowView<T, kShifted> view(first_row, a.rows, a.row_size);
+  const auto Slot = [&](int stage, int input, int j) {
+    return ring + ((stage * 3 + input) * kPacks + j) * blockDim.x + threadIdx.x;
+  };
+  const auto Ask = [&](int stage, int ahead) {
+    if (row + ahead * step < a.rows) {
+      RowView<T, kShifted> at = view;
+      at.first += ahead * jump;
 #pragma unroll
       for (int j = 0; j < kPacks; ++j) {
         const int p = t + j * a.group;
         if (p < view.packs) {
-          s[j] = view.Load(a.sum, p);
-          dy[j] = view.Load(a.dy, p);
-          if (a.dsum != nullptr) ds[j] = view.Load(a.dsum, p);
+          at.Copy(Slot(stage, 0, j), a.sum, p);
+          at.Copy(Slot(stage, 1, j), a.dy, p);
+          if (a.dsum != nullptr) at.Copy(Slot(stage, 2, j), a.dsum, p);
         }
       }
     }
+    CopyCommit();
+  };
+  const auto Values = [&](int stage, int input, int j, int p, float (&v)[kVec]) {
+    const uint4 w = *Slot(stage, input, j);
+    float2 f[kVec / 2];
+    WidenPack<kVec>(*reinterpret_cast<const P*>(&w), f);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      v[e] = e % 2 == 0 ? f[e / 2].x : f[e / 2].y;
+      if (view.Edge(p) && !view.Inside(p, e)) v[e] = 0.0f;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) Ask(i, i);
+  float inv_next = row < a.rows ? a.inv[row] : 0.0f;
+  float acc[kPacks][kVec];
+  P gamma[kPacks];
+#pragma unroll
+  for (int j = 0; j < kPacks; ++j) {
+    const int p = t + j * a.group;
+    if (p < view.packs) gamma[j] = view.Vector(a.gamma, p);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) acc[j][e] = 0.0f;
+  }
+  int stage = 0, parity = 0;
+  // Whole CTAs go round: the reductions of wide groups are barriers.
+  for (int64_t at = static_cast<int64_t>(blockIdx.x) * lanes; at < a.rows; at += step) {
+    const bool there = row < a.rows;
+    const float inv = inv_next;
+    if (row + step < a.rows) inv_next = a.inv[row + step];
+    CopyWait<kStages - 1>();
     float dot = 0.0f;
 #pragma unroll
     for (int j = 0; j < kPacks; ++j) {
       const int p = t + j * a.group;
       if (there && p < view.packs) {
-        const P gamma = view.Vector(a.gamma, p);
+        float s[kVec], dy[kVec];
+        Values(stage, 0, j, p, s);
+        Values(stage, 1, j, p, dy);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          if (view.Edge(p) && !view.Inside(p, e)) {
-            s[j].v[e] = FromF32<T>(0.0f);
-            dy[j].v[e] = FromF32<T>(0.0f);
-          }
-          const float dh = ToF32(dy[j].v[e]) * (ToF32(s[j].v[e]) * inv);
+          const float dh = dy[e] * (s[e] * inv);
           acc[j][e] += dh;
-          dot = fmaf(dh, ToF32(gamma.v[e]), dot);
+          dot = fmaf(dh, ToF32(gamma[j].v[e]), dot);
         }
       }
     }
     unsigned none = 0;
-    GroupSumMax(dot, none, a.group, sums[parity], tops[parity]);
+    GroupSumMax<false>(dot, none, a.group, sums[parity], nullptr);
     parity ^= 1;
-    const float mean = dot / a.row_size;
+    const float mean = dot * a.inv_size;
 #pragma unroll
     for (int j = 0; j < kPacks; ++j) {
       const int p = t + j * a.group;
       if (there && p < view.packs) {
-        const P gamma = view.Vector(a.gamma, p);
+        float s[kVec], d[kVec], past[kVec];
+        Values(stage, 0, j, p, s);
+        Values(stage, 1, j, p, d);
+        if (a.dsum != nullptr) Values(stage, 2, j, p, past);
         P out;
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          const float g = ToF32(dy[j].v[e]) * ToF32(gamma.v[e]);
-          float d = inv * (g - ToF32(s[j].v[e]) * inv * mean);
-          if (a.dsum != nullptr) d += ToF32(ds[j].v[e]);
-          out.v[e] = FromF32<T>(d);
+          float v = inv * (d[e] * ToF32(gamma[j].v[e]) - s[e] * inv * mean);
+          if (a.dsum != nullptr) v += past[e];
+          out.v[e] = FromF32<T>(v);
         }
         view.Store(a.dx, p, out);
       }
     }
+    Ask(stage, kStages);
+    if (++stage == kStages) stage = 0;
+    view.first += jump;
+    row += step;
   }
   float* partial = a.partial + static_cast<int64_t>(blockIdx.x) * a.row_size;
-  const RowView<T, kShifted> view(first_row, a.rows, a.row_size);
   if (lanes == 1) {
 #pragma unroll
     for (int j = 0; j < kPacks; ++j) {
@@ -383,6 +502,10 @@ __global__ void __launch_bounds__(kGradThreads) AddNormGradKernel(AddNormGradArg
     }
     return;
   }
+  // Over the ring: every copy of this CTA has landed and been read.
+  float* columns = reinterpret_cast<float*>(ring);
+  CopyWait<0>();
+  __syncthreads();
   for (int c = threadIdx.x; c < a.row_size; c += blockDim.x) columns[c] = 0.0f;
   __syncthreads();
   for (int l = 0; l < lanes; ++l) {
@@ -404,7 +527,8 @@ __global__ void __launch_bounds__(kGradThreads) AddNormGradKernel(AddNormGradArg
 template <typename T>
 __global__ void __launch_bounds__(kLoopThreads) AddNormGradLoopKernel(AddNormGradArgs a) {
   __shared__ float sums[2][32];
-  __shared__ unsigned tops[2][32];
+  GridDepWait();
+  GridDepLaunch();
   const T* gamma = static_cast<const T*>(a.gamma);
   float* partial = a.partial + static_cast<int64_t>(blockIdx.x) * a.row_size;
   for (int c = threadIdx.x; c < a.row_size; c += kLoopThreads) partial[c] = 0.0f;
@@ -420,9 +544,9 @@ __global__ void __launch_bounds__(kLoopThreads) AddNormGradLoopKernel(AddNormGra
       dot = fmaf(dh, ToF32(gamma[c]), dot);
     }
     unsigned none = 0;
-    GroupSumMax(dot, none, kLoopThreads, sums[parity], tops[parity]);
+    GroupSumMax<false>(dot, none, kLoopThreads, sums[parity], nullptr);
     parity ^= 1;
-    const float mean = dot / a.row_size;
+    const float mean = dot * a.inv_size;
     for (int c = threadIdx.x; c < a.row_size; c += kLoopThreads) {
       const int64_t at = row * a.row_size + c;
       float d = inv * (ToF32(dy[c]) * ToF32(gamma[c]) - ToF32(s[c]) * inv * mean);
@@ -444,32 +568,69 @@ int PowerOfTwoAtLeast(int64_t v, int low) {
   return p;
 }
 
+// CTAs that go round `rows` rows, `lanes` at a time, at most `most`: as even as the rounds
+// allow, and a multiple of `multiple` where a CTA has more than one round.
+int EvenCtas(int64_t rows, int lanes, int64_t most, int multiple) {
+  const int64_t blocks = CeilDiv(rows, lanes);
+  if (blocks <= most) return static_cast<int>(blocks);
+  const int64_t rounds = CeilDiv(blocks, most);
+  const int64_t even = CeilDiv(CeilDiv(blocks, rounds), multiple) * multiple;
+  return static_cast<int>(even <= most ? even : most / multiple * multiple);
+}
+
+// Function attributes are per device: raised once for each kernel.
+template <typename K>
+void AllowShared(std::atomic<int>* ready, K kernel) {
+  PerDevice(ready, [kernel] {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                200 * 1024) == cudaSuccess
+               ? 1
+               : 0;
+  });
+}
+
+template <typename T, int kPacks, bool kQuantize, bool kShifted>
+cudaError_t RunForward(const AddNormArgs& a, cudaStream_t stream) {
+  const int threads = a.group > 256 ? a.group : 256;
+  static std::atomic<int> ready[kMaxDevices];
+  AllowShared(ready, AddNormKernel<T, kPacks, kQuantize, kShifted>);
+  const int ctas = EvenCtas(a.rows, threads / a.group, SmCount() * (1024 / threads),
+                            kShifted ? VecWidth<T>::value : 1);
+  return LaunchChained(true, AddNormKernel<T, kPacks, kQuantize, kShifted>,
+                       dim3(static_cast<unsigned>(ctas)), dim3(threads),
+                       ForwardStages(kPacks) * 2 * kPacks * threads * 16, stream, a);
+}
+
 template <typename T, bool kQuantize>
 int LaunchForward(AddNormArgs a, bool aligned, cudaStream_t stream) {
   constexpr int kVec = VecWidth<T>::value;
+  // Four packs a thread where their sums fit 64 registers: fp32.
+  constexpr int kMost = sizeof(T) == 4 ? 4 : 2;
   const bool shifted = a.row_size % kVec != 0;
   const int64_t packs = CeilDiv(a.row_size, kVec) + (shifted ? 1 : 0);
-  CountKernelLaunch();
-  if (!aligned || packs > 4 * 1024) {
+  a.inv_size = 1.0f / a.row_size;
+  if (!aligned || packs > kMost * 1024) {
     const int64_t ctas = a.rows < SmCount() * 4 ? a.rows : SmCount() * 4;
-    AddNormLoopKernel<T, kQuantize><<<static_cast<unsigned>(ctas), kLoopThreads, 0, stream>>>(a);
-    return static_cast<int>(cudaGetLastError());
+    return static_cast<int>(LaunchChained(true, AddNormLoopKernel<T, kQuantize>,
+                                          dim3(static_cast<unsigned>(ctas)), dim3(kLoopThreads),
+                                          0, stream, a));
   }
   // Two packs a thread; one where rows are few (a call is all latency), four where a row
   // needs them.
-  int per_thread = a.rows <= SmCount() ? 1 : 2;
-  if (packs > per_thread * 1024) per_thread = packs > 2048 ? 4 : 2;
+  const int per_thread = packs > 2048 ? 4 : a.rows <= SmCount() && packs <= 1024 ? 1 : 2;
   a.group = PowerOfTwoAtLeast(CeilDiv(packs, per_thread), 8);
-  const int threads = a.group > 256 ? a.group : 256;
-  const dim3 grid(static_cast<unsigned>(CeilDiv(a.rows, threads / a.group)));
-#define MUSA_RUN(PACKS)                                                        \
-  (shifted ? AddNormKernel<T, PACKS, kQuantize, true><<<grid, threads, 0, stream>>>(a) \
-           : AddNormKernel<T, PACKS, kQuantize, false><<<grid, threads, 0, stream>>>(a))
-  if (per_thread == 1) MUSA_RUN(1);
-  else if (per_thread == 2) MUSA_RUN(2);
-  else MUSA_RUN(4);
-#undef MUSA_RUN
-  return static_cast<int>(cudaGetLastError());
+  cudaError_t rc;
+  if (per_thread == 1) {
+    rc = shifted ? RunForward<T, 1, kQuantize, true>(a, stream)
+                 : RunForward<T, 1, kQuantize, false>(a, stream);
+  } else if (per_thread == 2) {
+    rc = shifted ? RunForward<T, 2, kQuantize, true>(a, stream)
+                 : RunForward<T, 2, kQuantize, false>(a, stream);
+  } else {
+    rc = shifted ? RunForward<T, kMost, kQuantize, true>(a, stream)
+                 : RunForward<T, kMost, kQuantize, false>(a, stream);
+  }
+  return static_cast<int>(rc);
 }
 
 // The most CTAs of a gradient, a multiple of eight: their partial rows stay below 64 MB (or
@@ -480,39 +641,47 @@ int MostGradCtas(int64_t row_size) {
   return most < 8 ? 8 : static_cast<int>(most / 8 * 8);
 }
 
+template <typename T, int kPacks, int kThreads, bool kShifted>
+cudaError_t RunGrad(const AddNormGradArgs& a, int most, int* ctas, cudaStream_t stream) {
+  const int threads = kThreads == 256 ? 256 : a.group;
+  static std::atomic<int> ready[kMaxDevices];
+  AllowShared(ready, AddNormGradKernel<T, kPacks, kThreads, kShifted>);
+  const int resident = SmCount() * (kThreads == 256 ? GradCtas(256) : 1024 / threads);
+  *ctas = EvenCtas(a.rows, threads / a.group, resident < most ? resident : most,
+                   kShifted ? VecWidth<T>::value : 1);
+  return LaunchChained(true, AddNormGradKernel<T, kPacks, kThreads, kShifted>, dim3(*ctas),
+                       dim3(threads), GradStages(kPacks, kThreads) * 3 * kPacks * threads * 16,
+                       stream, a);
+}
+
 template <typename T>
 int LaunchGrad(AddNormGradArgs a, bool aligned, void* dgamma, cudaStream_t stream) {
   constexpr int kVec = VecWidth<T>::value;
+  constexpr int kMost = sizeof(T) == 4 ? 4 : 2;
   const bool shifted = a.row_size % kVec != 0;
   const int64_t packs = CeilDiv(a.row_size, kVec) + (shifted ? 1 : 0);
   const int most = MostGradCtas(a.row_size);
   int ctas;
-  CountKernelLaunch();
-  if (!aligned || packs > 4 * kGradThreads) {
+  cudaError_t rc;
+  a.inv_size = 1.0f / a.row_size;
+  if (!aligned || packs > kMost * 1024) {
     ctas = static_cast<int>(a.rows < most ? a.rows : most);
-    AddNormGradLoopKernel<T><<<ctas, kLoopThreads, 0, stream>>>(a);
+    rc = LaunchChained(true, AddNormGradLoopKernel<T>, dim3(ctas), dim3(kLoopThreads), 0, stream,
+                       a);
   } else {
-    const int per_thread = packs > 2 * kGradThreads ? 4 : 2;
+    const int per_thread = packs > 2048 ? 4 : 2;
     a.group = PowerOfTwoAtLeast(CeilDiv(packs, per_thread), 8);
-    const int threads = a.group > 256 ? a.group : 256;
-    const int lanes = threads / a.group;
-    int64_t want = CeilDiv(a.rows, lanes);
-    if (want > most) want = most;
-    // Shifted rows: a thread's rows are a multiple of the pack width apart.
-    if (shifted && want * lanes < a.rows) want = want / kVec * kVec;
-    ctas = static_cast<int>(want);
-    const size_t smem = lanes > 1 ? sizeof(float) * a.row_size : 0;
-#define MUSA_RUN(PACKS)                                                              \
-  (shifted ? AddNormGradKernel<T, PACKS, true><<<ctas, threads, smem, stream>>>(a)   \
-           : AddNormGradKernel<T, PACKS, false><<<ctas, threads, smem, stream>>>(a))
-    if (per_thread == 2) MUSA_RUN(2);
-    else MUSA_RUN(4);
+#define MUSA_RUN(PACKS, THREADS)                                           \
+  (shifted ? RunGrad<T, PACKS, THREADS, true>(a, most, &ctas, stream)      \
+           : RunGrad<T, PACKS, THREADS, false>(a, most, &ctas, stream))
+    rc = a.group <= 256    ? MUSA_RUN(2, 256)
+         : per_thread == 2 ? MUSA_RUN(2, 1024)
+                           : MUSA_RUN(kMost, 1024);
 #undef MUSA_RUN
   }
-  const cudaError_t rc = cudaGetLastError();
   if (rc != cudaSuccess) return static_cast<int>(rc);
   return static_cast<int>(
-      LaunchAddPartialRows<T>(false, a.partial, ctas, a.row_size, dgamma, stream));
+      LaunchAddPartialRows<T>(true, a.partial, ctas, a.row_size, dgamma, stream));
 }
 
 template <typename T>
@@ -528,7 +697,7 @@ int AddNorm(const void* x, const void* residual, const void* gamma, void* y, voi
   const bool aligned = Aligned16(x) && Aligned16(residual) && Aligned16(gamma) && Aligned16(y) &&
                        Aligned16(sum);
   return LaunchForward<T, false>({x, residual, gamma, y, sum, inv_rms, rows,
-                                  static_cast<int>(row_size), 0, epsilon},
+                                  static_cast<int>(row_size), 0, epsilon, 0.0f},
                                  aligned, stream);
 }
 
@@ -547,7 +716,7 @@ int AddNormQuantize(const void* x, const void* residual, const void* gamma, void
   const bool aligned = Aligned16(x) && Aligned16(residual) && Aligned16(gamma) && Aligned16(q) &&
                        Aligned16(sum);
   return LaunchForward<T, true>({x, residual, gamma, q, sum, scale, rows,
-                                 static_cast<int>(row_size), 0, epsilon},
+                                 static_cast<int>(row_size), 0, epsilon, 0.0f},
                                 aligned, stream);
 }
 
@@ -572,7 +741,7 @@ int AddNormGrad(const void* dy, const void* dsum, const void* sum, const float* 
   const bool aligned = Aligned16(dy) && Aligned16(dsum) && Aligned16(sum) && Aligned16(gamma) &&
                        Aligned16(dx);
   return LaunchGrad<T>({dy, dsum, sum, inv_rms, gamma, dx, static_cast<float*>(workspace), rows,
-                        static_cast<int>(row_size), 0},
+                        static_cast<int>(row_size), 0, 0.0f},
                        aligned, dgamma, stream);
 }
 
