@@ -80,21 +80,20 @@ __device__ __forceinline__ float QuantizeScale(float top) {
   return t < kScaleMin ? kScaleMin : t;  // NaN goes through
 }
 
-// y / scale.  Rows quantised as they are take the rounded division: quotients of 16-bit
-// values fall on borders between two e4m3 values, where a last bit decides.  Behind a norm
-// the fp32 values are off by more than the product with the reciprocal.
-__device__ __forceinline__ float Quotient(float y, float scale, float unscale, bool normed) {
-  return normed ? y * unscale : y / scale;
+// The larger of `w` and |v|; NaN stays.
+__device__ __forceinline__ float MaxMagnitude(float w, float v) {
+  float out;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(out) : "f"(w), "f"(fabsf(v)));
+  return out;
 }
 
 template <int kVec>
-__device__ __forceinline__ Pack<uint8_t, kVec> ToE4m3(const float (&v)[kVec]) {
+__device__ __forceinline__ Pack<uint8_t, kVec> ToE4m3(const float2 (&v)[kVec / 2]) {
   Pack<uint8_t, kVec> out;
   uint16_t* w = reinterpret_cast<uint16_t*>(&out);
 #pragma unroll
   for (int i = 0; i < kVec / 2; ++i) {
-    w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE,
-                                    __NV_E4M3);
+    w[i] = __nv_cvt_float2_to_fp8x2(v[i], __NV_SATFINITE, __NV_E4M3);
   }
   return out;
 }
@@ -144,6 +143,16 @@ struct RowView {
   __device__ bool Edge(int p) const { return kShifted && (p == 0 || p == packs - 1); }
   __device__ bool Inside(int p, int e) const {
     return static_cast<unsigned>(p * kVec + e - shift) < static_cast<unsigned>(row_size);
+  }
+  // Elements of other rows become zeros.
+  __device__ void Mask(int p, float2 (&v)[kVec / 2]) const {
+    if (Edge(p)) {
+#pragma unroll
+      for (int e = 0; e < kVec / 2; ++e) {
+        if (!Inside(p, 2 * e)) v[e].x = 0.0f;
+        if (!Inside(p, 2 * e + 1)) v[e].y = 0.0f;
+      }
+    }
   }
   // Starts the copy of pack p to a slot of shared memory; what lies behind the tensor is
   // not read and comes as zeros.
@@ -209,6 +218,10 @@ __global__ void __launch_bounds__(1024) AddNormKernel(AddNormArgs a) {
   int64_t row = base + threadIdx.x / a.group;
   RowView<T, kShifted> view(row, a.rows, a.row_size);
   const int64_t jump = step * a.row_size;
+  const auto Widen = [](const uint4* slot, float2 (&v)[kVec / 2]) {
+    const uint4 w = *slot;
+    WidenPack<kVec>(*reinterpret_cast<const P*>(&w), v);
+  };
   const auto Slot = [&](int stage, int input, int j) {
     return ring + ((stage * 2 + input) * kPacks + j) * blockDim.x + threadIdx.x;
   };
@@ -241,37 +254,37 @@ __global__ void __launch_bounds__(1024) AddNormKernel(AddNormArgs a) {
   for (int64_t at = base; at < a.rows; at += step) {
     const bool there = row < a.rows;
     CopyWait<kStages - 1>();
-    float s[kPacks][kVec];
-    float square = 0.0f;
-    unsigned top = 0;
+    float2 s[kPacks][kVec / 2];
+    float2 squares = make_float2(0.0f, 0.0f);
+    float largest = 0.0f;
 #pragma unroll
     for (int j = 0; j < kPacks; ++j) {
       const int p = t + j * a.group;
       if (there && p < view.packs) {
-        const uint4 xw = *Slot(stage, 0, j);
-        float2 x[kVec / 2];
-        WidenPack<kVec>(*reinterpret_cast<const P*>(&xw), x);
+        Widen(Slot(stage, 0, j), s[j]);
         if (add) {
-          const uint4 rw = *Slot(stage, 1, j);
           float2 r[kVec / 2];
-          WidenPack<kVec>(*reinterpret_cast<const P*>(&rw), r);
+          Widen(Slot(stage, 1, j), r);
 #pragma unroll
-          for (int e = 0; e < kVec / 2; ++e) x[e] = Add2(x[e], r[e]);
+          for (int e = 0; e < kVec / 2; ++e) s[j][e] = Add2(s[j][e], r[e]);
         }
+        view.Mask(p, s[j]);
+        float2 g[kVec / 2];
+        if (kQuantize && normed) WidenPack<kVec>(gamma[j], g);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          s[j][e] = e % 2 == 0 ? x[e / 2].x : x[e / 2].y;
-          if (view.Edge(p) && !view.Inside(p, e)) s[j][e] = 0.0f;
-          square = fmaf(s[j][e], s[j][e], square);
+        for (int e = 0; e < kVec / 2; ++e) {
+          squares = Fma2(s[j][e], s[j][e], squares);
           if constexpr (kQuantize) {
-            const float g = normed ? ToF32(gamma[j].v[e]) : 1.0f;
-            top = max(top, MagnitudeBits(s[j][e] * g));
+            const float2 v = normed ? Mul2(s[j][e], g[e]) : s[j][e];
+            largest = MaxMagnitude(MaxMagnitude(largest, v.x), v.y);
           }
         }
       }
     }
     Ask(stage, kStages);
     if (++stage == kStages) stage = 0;
+    float square = squares.x + squares.y;
+    unsigned top = MagnitudeBits(largest);
     GroupSumMax<kQuantize>(square, top, a.group, sums[parity], tops[parity]);
     parity ^= 1;
     float inv = rsqrtf(fmaf(square, a.inv_size, a.epsilon));
@@ -282,27 +295,39 @@ __global__ void __launch_bounds__(1024) AddNormKernel(AddNormArgs a) {
       unscale = 1.0f / scale;
     }
     if (there && t == 0) a.stat[row] = kQuantize ? scale : inv;
+    const float2 invs = make_float2(inv, inv), unscales = make_float2(unscale, unscale);
 #pragma unroll
     for (int j = 0; j < kPacks; ++j) {
       const int p = t + j * a.group;
       if (there && p < view.packs) {
-        P total;
-        float y[kVec];
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          total.v[e] = FromF32<T>(s[j][e]);
-          y[e] = s[j][e] * inv;
-          if (normed) y[e] *= ToF32(gamma[j].v[e]);
+        if (!kQuantize || a.sum != nullptr) {
+          P total;
+          NarrowPack<kVec>(s[j], total);
+          view.Store(a.sum, p, total);
         }
-        if (!kQuantize || a.sum != nullptr) view.Store(a.sum, p, total);
-        if constexpr (kQuantize) {
+        if (normed) {
+          float2 g[kVec / 2];
+          WidenPack<kVec>(gamma[j], g);
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) y[e] = Quotient(y[e], scale, unscale, normed);
-          view.Store(a.y, p, ToE4m3<kVec>(y));
+          for (int e = 0; e < kVec / 2; ++e) {
+            s[j][e] = Mul2(Mul2(s[j][e], invs), g[e]);
+            // Last: inv / scale alone passes the largest float in a row of zeros.
+            if (kQuantize) s[j][e] = Mul2(s[j][e], unscales);
+          }
+        } else {
+          // Rows as they are take the rounded division: quotients of 16-bit values fall on
+          // borders between two e4m3 values, where a last bit decides.  Behind a norm the
+          // fp32 values are off by more than the product with the reciprocal.
+#pragma unroll
+          for (int e = 0; e < kVec / 2; ++e) {
+            s[j][e] = make_float2(s[j][e].x / scale, s[j][e].y / scale);
+          }
+        }
+        if constexpr (kQuantize) {
+          view.Store(a.y, p, ToE4m3<kVec>(s[j]));
         } else {
           P out;
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) out.v[e] = FromF32<T>(y[e]);
+          NarrowPack<kVec>(s[j], out);
           view.Store(a.y, p, out);
         }
       }
@@ -348,7 +373,7 @@ __global__ void __launch_bounds__(kLoopThreads) AddNormLoopKernel(AddNormArgs a)
       const float y = s * inv * (gamma != nullptr ? ToF32(gamma[c]) : 1.0f);
       if constexpr (kQuantize) {
         static_cast<uint8_t*>(a.y)[at] =
-            __nv_cvt_float_to_fp8(Quotient(y, scale, unscale, gamma != nullptr), __NV_SATFINITE,
+            __nv_cvt_float_to_fp8(gamma != nullptr ? y * unscale : y / scale, __NV_SATFINITE,
                                   __NV_E4M3);
       } else {
         static_cast<T*>(a.y)[at] = FromF32<T>(y);
@@ -376,14 +401,17 @@ struct AddNormGradArgs {
 // As the forward, with the dgamma of a thread's columns in registers too; a row's slots are
 // read twice, before and after its reduction, and asked for again behind its stores.  At the
 // end the row lanes of the CTA are added in order and the CTA leaves one partial row.
+// Registers (85, 128 or 64) and shared memory (72, 96 or 192 KB) of the three shapes that the
+// launch takes: two packs for 256 threads, four for 256 and 512, fp32 rows of more for 1024.
 __host__ __device__ constexpr int GradStages(int packs, int threads) {
-  return packs == 4 ? 1 : threads == 1024 ? 2 : 3;
+  return packs == 2 ? 3 : threads == 1024 ? 1 : 2;
 }
-// CTAs per SM at the registers of 85 and the shared memory of three stages.
-__host__ __device__ constexpr int GradCtas(int threads) { return threads == 1024 ? 1 : 3; }
+__host__ __device__ constexpr int GradCtas(int packs, int threads) {
+  return threads > 256 ? 1 : packs == 2 ? 3 : 2;
+}
 
 template <typename T, int kPacks, int kThreads, bool kShifted>
-__global__ void __launch_bounds__(kThreads, GradCtas(kThreads)) AddNormGradKernel(
+__global__ void __launch_bounds__(kThreads, GradCtas(kPacks, kThreads)) AddNormGradKernel(
     AddNormGradArgs a) {
   constexpr int kVec = VecWidth<T>::value;
   constexpr int kStages = GradStages(kPacks, kThreads);
@@ -418,27 +446,22 @@ __global__ void __launch_bounds__(kThreads, GradCtas(kThreads)) AddNormGradKerne
     }
     CopyCommit();
   };
-  const auto Values = [&](int stage, int input, int j, int p, float (&v)[kVec]) {
+  const auto Values = [&](int stage, int input, int j, int p, float2 (&v)[kVec / 2]) {
     const uint4 w = *Slot(stage, input, j);
-    float2 f[kVec / 2];
-    WidenPack<kVec>(*reinterpret_cast<const P*>(&w), f);
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      v[e] = e % 2 == 0 ? f[e / 2].x : f[e / 2].y;
-      if (view.Edge(p) && !view.Inside(p, e)) v[e] = 0.0f;
-    }
+    WidenPack<kVec>(*reinterpret_cast<const P*>(&w), v);
+    view.Mask(p, v);
   };
 #pragma unroll
   for (int i = 0; i < kStages; ++i) Ask(i, i);
   float inv_next = row < a.rows ? a.inv[row] : 0.0f;
-  float acc[kPacks][kVec];
+  float2 acc[kPacks][kVec / 2];
   P gamma[kPacks];
 #pragma unroll
   for (int j = 0; j < kPacks; ++j) {
     const int p = t + j * a.group;
     if (p < view.packs) gamma[j] = view.Vector(a.gamma, p);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) acc[j][e] = 0.0f;
+    for (int e = 0; e < kVec / 2; ++e) acc[j][e] = make_float2(0.0f, 0.0f);
   }
   int stage = 0, parity = 0;
   // Whole CTAs go round: the reductions of wide groups are barriers.
@@ -447,41 +470,50 @@ __global__ void __launch_bounds__(kThreads, GradCtas(kThreads)) AddNormGradKerne
     const float inv = inv_next;
     if (row + step < a.rows) inv_next = a.inv[row + step];
     CopyWait<kStages - 1>();
-    float dot = 0.0f;
+    float2 dots = make_float2(0.0f, 0.0f);
+    const float2 invs = make_float2(inv, inv);
 #pragma unroll
     for (int j = 0; j < kPacks; ++j) {
       const int p = t + j * a.group;
       if (there && p < view.packs) {
-        float s[kVec], dy[kVec];
+        float2 s[kVec / 2], dy[kVec / 2], g[kVec / 2];
         Values(stage, 0, j, p, s);
         Values(stage, 1, j, p, dy);
+        WidenPack<kVec>(gamma[j], g);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const float dh = dy[e] * (s[e] * inv);
-          acc[j][e] += dh;
-          dot = fmaf(dh, ToF32(gamma[j].v[e]), dot);
+        for (int e = 0; e < kVec / 2; ++e) {
+          const float2 dh = Mul2(dy[e], Mul2(s[e], invs));
+          acc[j][e] = Add2(acc[j][e], dh);
+          dots = Fma2(dh, g[e], dots);
         }
       }
     }
+    float dot = dots.x + dots.y;
     unsigned none = 0;
     GroupSumMax<false>(dot, none, a.group, sums[parity], nullptr);
     parity ^= 1;
-    const float mean = dot * a.inv_size;
+    // dx = dsum + inv * (g - h * mean), h = s * inv.
+    const float back = -inv * inv * (dot * a.inv_size);
+    const float2 backs = make_float2(back, back);
 #pragma unroll
     for (int j = 0; j < kPacks; ++j) {
       const int p = t + j * a.group;
       if (there && p < view.packs) {
-        float s[kVec], d[kVec], past[kVec];
+        float2 s[kVec / 2], dy[kVec / 2], g[kVec / 2];
         Values(stage, 0, j, p, s);
-        Values(stage, 1, j, p, d);
-        if (a.dsum != nullptr) Values(stage, 2, j, p, past);
-        P out;
+        Values(stage, 1, j, p, dy);
+        WidenPack<kVec>(gamma[j], g);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          float v = inv * (d[e] * ToF32(gamma[j].v[e]) - s[e] * inv * mean);
-          if (a.dsum != nullptr) v += past[e];
-          out.v[e] = FromF32<T>(v);
+        for (int e = 0; e < kVec / 2; ++e) {
+          s[e] = Fma2(Mul2(dy[e], g[e]), invs, Mul2(s[e], backs));
         }
+        if (a.dsum != nullptr) {
+          Values(stage, 2, j, p, dy);
+#pragma unroll
+          for (int e = 0; e < kVec / 2; ++e) s[e] = Add2(s[e], dy[e]);
+        }
+        P out;
+        NarrowPack<kVec>(s, out);
         view.Store(a.dx, p, out);
       }
     }
@@ -497,7 +529,9 @@ __global__ void __launch_bounds__(kThreads, GradCtas(kThreads)) AddNormGradKerne
       const int p = t + j * a.group;
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        if (p < view.packs && view.Inside(p, e)) partial[p * kVec + e - view.shift] = acc[j][e];
+        if (p < view.packs && view.Inside(p, e)) {
+          partial[p * kVec + e - view.shift] = e % 2 == 0 ? acc[j][e / 2].x : acc[j][e / 2].y;
+        }
       }
     }
     return;
@@ -515,7 +549,9 @@ __global__ void __launch_bounds__(kThreads, GradCtas(kThreads)) AddNormGradKerne
         const int p = t + j * a.group;
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          if (p < view.packs && view.Inside(p, e)) columns[p * kVec + e - view.shift] += acc[j][e];
+          if (p < view.packs && view.Inside(p, e)) {
+            columns[p * kVec + e - view.shift] += e % 2 == 0 ? acc[j][e / 2].x : acc[j][e / 2].y;
+          }
         }
       }
     }
@@ -643,10 +679,10 @@ int MostGradCtas(int64_t row_size) {
 
 template <typename T, int kPacks, int kThreads, bool kShifted>
 cudaError_t RunGrad(const AddNormGradArgs& a, int most, int* ctas, cudaStream_t stream) {
-  const int threads = kThreads == 256 ? 256 : a.group;
+  constexpr int threads = kThreads;
   static std::atomic<int> ready[kMaxDevices];
   AllowShared(ready, AddNormGradKernel<T, kPacks, kThreads, kShifted>);
-  const int resident = SmCount() * (kThreads == 256 ? GradCtas(256) : 1024 / threads);
+  const int resident = SmCount() * GradCtas(kPacks, kThreads);
   *ctas = EvenCtas(a.rows, threads / a.group, resident < most ? resident : most,
                    kShifted ? VecWidth<T>::value : 1);
   return LaunchChained(true, AddNormGradKernel<T, kPacks, kThreads, kShifted>, dim3(*ctas),
@@ -657,26 +693,28 @@ cudaError_t RunGrad(const AddNormGradArgs& a, int most, int* ctas, cudaStream_t 
 template <typename T>
 int LaunchGrad(AddNormGradArgs a, bool aligned, void* dgamma, cudaStream_t stream) {
   constexpr int kVec = VecWidth<T>::value;
-  constexpr int kMost = sizeof(T) == 4 ? 4 : 2;
+  // 1024 threads of four packs where their sums fit 64 registers: fp32.
+  constexpr int kWidest = sizeof(T) == 4 ? 1024 : 512;
   const bool shifted = a.row_size % kVec != 0;
   const int64_t packs = CeilDiv(a.row_size, kVec) + (shifted ? 1 : 0);
   const int most = MostGradCtas(a.row_size);
   int ctas;
   cudaError_t rc;
   a.inv_size = 1.0f / a.row_size;
-  if (!aligned || packs > kMost * 1024) {
+  if (!aligned || packs > 4 * kWidest) {
     ctas = static_cast<int>(a.rows < most ? a.rows : most);
     rc = LaunchChained(true, AddNormGradLoopKernel<T>, dim3(ctas), dim3(kLoopThreads), 0, stream,
                        a);
   } else {
-    const int per_thread = packs > 2048 ? 4 : 2;
+    const int per_thread = packs > 512 ? 4 : 2;
     a.group = PowerOfTwoAtLeast(CeilDiv(packs, per_thread), 8);
 #define MUSA_RUN(PACKS, THREADS)                                           \
   (shifted ? RunGrad<T, PACKS, THREADS, true>(a, most, &ctas, stream)      \
            : RunGrad<T, PACKS, THREADS, false>(a, most, &ctas, stream))
-    rc = a.group <= 256    ? MUSA_RUN(2, 256)
-         : per_thread == 2 ? MUSA_RUN(2, 1024)
-                           : MUSA_RUN(kMost, 1024);
+    rc = per_thread == 2  ? MUSA_RUN(2, 256)
+         : a.group <= 256 ? MUSA_RUN(4, 256)
+         : a.group <= 512 ? MUSA_RUN(4, 512)
+                          : MUSA_RUN(4, kWidest);
 #undef MUSA_RUN
   }
   if (rc != cudaSuccess) return static_cast<int>(rc);
