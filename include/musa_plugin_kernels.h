@@ -522,8 +522,9 @@ int LaunchMatMulBiasAct(int dtype, const void* a, int64_t lda, bool transpose_a,
  * of the residual is dy.  da, db and dbias may be null; preactivation is not read with
  * MUSA_ACT_IDENTITY. */
 size_t MatMulGradWorkspaceBytes(const void* dy, const void* a, int64_t lda, bool transpose_a,
-                                const void* b, int64_t ldb, bool transpose_b, int64_t m,
-                                int64_t n, int64_t k, int act);
+                                const void* b, int64_t ldb, bool transpose_b,
+                                const void* preactivation, int64_t m, int64_t n, int64_t k,
+                                int act);
 int LaunchMatMulBiasActGrad(int dtype, const void* dy, const void* a, int64_t lda,
                             bool transpose_a, const void* b, int64_t ldb, bool transpose_b,
                             const void* preactivation, void* da, void* db, void* dbias,

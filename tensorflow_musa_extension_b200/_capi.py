@@ -154,7 +154,7 @@ PROTOTYPES.update({
     "MatMulWorkspaceBytes": (c_size, [c_int] + _FACTORS + [c_i64] * 3),
     "LaunchMatMulBiasAct":
         (c_int, [c_int] + _FACTORS + [c_vp] * 4 + [c_i64] * 3 + [c_int, c_vp, c_size, c_vp]),
-    "MatMulGradWorkspaceBytes": (c_size, [c_vp] + _FACTORS + [c_i64] * 3 + [c_int]),
+    "MatMulGradWorkspaceBytes": (c_size, [c_vp] + _FACTORS + [c_vp] + [c_i64] * 3 + [c_int]),
     "LaunchMatMulBiasActGrad":
         (c_int, [c_int, c_vp] + _FACTORS + [c_vp] * 4 + [c_i64] * 3
          + [c_int, c_vp, c_size, c_vp]),

@@ -723,6 +723,8 @@ template <typename E>
 __global__ void __launch_bounds__(256)
     RepitchKernel(const E* __restrict__ src, E* __restrict__ dst, int64_t lines, int64_t columns,
                   int64_t ld, int64_t pitch) {
+  GridDepWait();
+  GridDepLaunch();
   for (int64_t r = blockIdx.y; r < lines; r += gridDim.y) {
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x;
 #pragma unroll
@@ -762,19 +764,18 @@ cudaError_t Repitch(Factor* f, int64_t rows, int64_t depth, int elem, uint8_t** 
   const int64_t pitch = RoundUp(l.length * elem, 16) / elem;
   const dim3 grid(static_cast<unsigned>(CeilDiv(l.length, 1024)),
                   static_cast<unsigned>(l.count < 32768 ? l.count : 32768));
-  CountKernelLaunch();
-  if (elem == 2) {
-    RepitchKernel<uint16_t><<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(f->p),
-                                                      reinterpret_cast<uint16_t*>(*workspace),
-                                                      l.count, l.length, f->ld, pitch);
-  } else {
-    RepitchKernel<uint8_t><<<grid, 256, 0, stream>>>(static_cast<const uint8_t*>(f->p),
-                                                     *workspace, l.count, l.length, f->ld, pitch);
-  }
+  const cudaError_t rc =
+      elem == 2 ? LaunchChained(true, RepitchKernel<uint16_t>, grid, dim3(256), 0, stream,
+                                static_cast<const uint16_t*>(f->p),
+                                reinterpret_cast<uint16_t*>(*workspace), l.count, l.length, f->ld,
+                                pitch)
+                : LaunchChained(true, RepitchKernel<uint8_t>, grid, dim3(256), 0, stream,
+                                static_cast<const uint8_t*>(f->p), *workspace, l.count, l.length,
+                                f->ld, pitch);
   f->p = *workspace;
   f->ld = pitch;
   *workspace += RoundUp(static_cast<int64_t>(bytes), 16);
-  return cudaGetLastError();
+  return rc;
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -998,14 +999,20 @@ struct SlopeArgs {
   int act;
 };
 
+constexpr int kSumCtas = 3;      // per SM: one wave of them, 85 registers
+
 template <typename T, int kVec>
-__global__ void __launch_bounds__(32 * kSumRows) SlopeKernel(SlopeArgs a) {
+__global__ void __launch_bounds__(32 * kSumRows, kSumCtas) SlopeKernel(SlopeArgs a) {
   using P = Pack<T, kVec>;
+  constexpr int kUnroll = 4;
   __shared__ float sums[kSumRows][32 * kVec + 1];
+  GridDepWait();
+  GridDepLaunch();
   const int lane = threadIdx.x % 32, row_lane = threadIdx.x / 32;
   const int64_t col = (static_cast<int64_t>(blockIdx.x) * 32 + lane) * kVec;
   const int64_t begin = blockIdx.y * a.rows_per_cta;
   const int64_t end = begin + a.rows_per_cta < a.m ? begin + a.rows_per_cta : a.m;
+  const bool bent = a.act != MUSA_ACT_IDENTITY;
   float sum[kVec];
 #pragma unroll
   for (int e = 0; e < kVec; ++e) sum[e] = 0.0f;
@@ -1013,33 +1020,40 @@ __global__ void __launch_bounds__(32 * kSumRows) SlopeKernel(SlopeArgs a) {
     const T* dy = static_cast<const T*>(a.dy) + col;
     const T* z = static_cast<const T*>(a.z) + col;
     T* dz = static_cast<T*>(a.dz) + col;
-#pragma unroll 4
-    for (int64_t r = begin + row_lane; r < end; r += kSumRows) {
-      const P g = LoadStream(reinterpret_cast<const P*>(dy + r * a.n));
-      P out;
-      if (a.act != MUSA_ACT_IDENTITY) {
-        const P x = LoadStream(reinterpret_cast<const P*>(z + r * a.n));
+    for (int64_t r = begin + row_lane; r < end; r += kSumRows * kUnroll) {
+      P g[kUnroll], x[kUnroll];
 #pragma unroll
-        for (int e = 0; e < kVec; e += 2) {
-          const int f = kVec > 1 ? e + 1 : e;
-          const float2 slope = Slope(make_float2(ToF32(x.v[e]), ToF32(x.v[f])), a.act);
-          const float d0 = ToF32(g.v[e]) * slope.x;
-          sum[e] += d0;
-          out.v[e] = FromF32<T>(d0);
-          if (kVec > 1) {
-            const float d1 = ToF32(g.v[f]) * slope.y;
-            sum[f] += d1;
-            out.v[f] = FromF32<T>(d1);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          sum[e] += ToF32(g.v[e]);
-          out.v[e] = g.v[e];
+      for (int u = 0; u < kUnroll; ++u) {
+        const int64_t row = r + u * kSumRows;
+        if (row < end) {
+          g[u] = LoadStream(reinterpret_cast<const P*>(dy + row * a.n));
+          if (bent) x[u] = LoadStream(reinterpret_cast<const P*>(z + row * a.n));
         }
       }
-      if (a.dz != nullptr) *reinterpret_cast<P*>(dz + r * a.pitch) = out;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int64_t row = r + u * kSumRows;
+        if (row >= end) break;
+        if (bent) {
+#pragma unroll
+          for (int e = 0; e < kVec; e += 2) {
+            const int f = kVec > 1 ? e + 1 : e;
+            const float2 slope = Slope(make_float2(ToF32(x[u].v[e]), ToF32(x[u].v[f])), a.act);
+            const float d0 = ToF32(g[u].v[e]) * slope.x;
+            sum[e] += d0;
+            g[u].v[e] = FromF32<T>(d0);
+            if (kVec > 1) {
+              const float d1 = ToF32(g[u].v[f]) * slope.y;
+              sum[f] += d1;
+              g[u].v[f] = FromF32<T>(d1);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) sum[e] += ToF32(g[u].v[e]);
+        }
+        if (a.dz != nullptr) *reinterpret_cast<P*>(dz + row * a.pitch) = g[u];
+      }
     }
   }
 #pragma unroll
@@ -1058,18 +1072,18 @@ struct SumShape {
   int64_t rows_per_cta;
   int parts;
 };
-// About four CTAs per SM over columns and rows, at least 64 rows each.
-SumShape SumRows(int64_t m, int64_t n) {
-  const int64_t blocks = n > 0 ? CeilDiv(n, 256) : 1;
-  int64_t parts = CeilDiv(4 * 148, blocks);
+// One wave of CTAs over blocks of `width` columns and parts of at least 64 rows.
+SumShape SumRows(int64_t m, int64_t n, int width) {
+  const int64_t blocks = n > 0 ? CeilDiv(n, width) : 1;
+  int64_t parts = static_cast<int64_t>(SmCount()) * kSumCtas / blocks;
   if (parts > CeilDiv(m, 64)) parts = CeilDiv(m, 64);
   if (parts < 1) parts = 1;
-  if (parts > 1024) parts = 1024;
   const int64_t rows = CeilDiv(CeilDiv(m, parts), kSumRows) * kSumRows;
   return {rows < 1 ? 1 : rows, static_cast<int>(rows < 1 ? 1 : CeilDiv(m, rows))};
 }
 
 struct GradPlan {
+  bool packed;         // whole 16-byte packs
   bool want_dz;        // dz goes to the workspace
   int64_t dz_pitch;
   SumShape sum;
@@ -1077,13 +1091,14 @@ struct GradPlan {
   size_t Total() const { return dz_bytes + partial_bytes + a_bytes + b_bytes + 64; }
 };
 
-GradPlan PlanGrad(const void* dy, const Factor& a, const Factor& b, int64_t m, int64_t n,
-                  int64_t k, int act) {
+GradPlan PlanGrad(const void* dy, const void* z, const Factor& a, const Factor& b, int64_t m,
+                  int64_t n, int64_t k, int act) {
   GradPlan p = {};
+  p.packed = n % 8 == 0 && Aligned16(dy) && Aligned16(z);
   const bool direct = act == MUSA_ACT_IDENTITY && Aligned16(dy) && n % 8 == 0;
   p.want_dz = !direct;
   p.dz_pitch = RoundUp(n, 8);
-  p.sum = SumRows(m, n);
+  p.sum = SumRows(m, n, p.packed ? 256 : 32);
   p.dz_bytes = p.want_dz ? static_cast<size_t>(RoundUp(p.dz_pitch * m * 2, 16)) : 0;
   p.partial_bytes = static_cast<size_t>(RoundUp(n * p.sum.parts * 4, 16));
   p.a_bytes = static_cast<size_t>(RoundUp(RepitchBytes(a, m, k, 2), 16));
@@ -1130,7 +1145,7 @@ template <typename T>
 int Backward(const void* dy, Factor a, Factor b, const void* z, void* da, void* db, void* dbias,
              int64_t m, int64_t n, int64_t k, int act, void* workspace, size_t bytes,
              cudaStream_t stream) {
-  const GradPlan p = PlanGrad(dy, a, b, m, n, k, act);
+  const GradPlan p = PlanGrad(dy, act == MUSA_ACT_IDENTITY ? nullptr : z, a, b, m, n, k, act);
   if (BadWorkspace(workspace, bytes, p.Total())) return MUSA_KERNELS_EWORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   float* partial = reinterpret_cast<float*>(ws);
@@ -1141,14 +1156,13 @@ int Backward(const void* dy, Factor a, Factor b, const void* z, void* da, void* 
   if (m > 0 && n > 0) {
     if (p.want_dz || dbias != nullptr) {
       SlopeArgs s = {dy, z, dz, partial, m, n, p.dz_pitch, p.sum.rows_per_cta, act};
-      const bool packed = n % 8 == 0 && Aligned16(dy) && (z == nullptr || Aligned16(z));
-      const dim3 grid(static_cast<unsigned>(CeilDiv(n, packed ? 256 : 32)),
+      const dim3 grid(static_cast<unsigned>(CeilDiv(n, p.packed ? 256 : 32)),
                       static_cast<unsigned>(p.sum.parts));
-      CountKernelLaunch();
-      if (packed) SlopeKernel<T, 8><<<grid, 32 * kSumRows, 0, stream>>>(s);
-      else SlopeKernel<T, 1><<<grid, 32 * kSumRows, 0, stream>>>(s);
+      rc = LaunchChained(true, p.packed ? SlopeKernel<T, 8> : SlopeKernel<T, 1>, grid,
+                         dim3(32 * kSumRows), 0, stream, s);
+      if (rc != cudaSuccess) return static_cast<int>(rc);
       if (dbias != nullptr) {
-        rc = LaunchAddPartialRows<T>(false, partial, p.sum.parts, n, dbias, stream);
+        rc = LaunchAddPartialRows<T>(true, partial, p.sum.parts, n, dbias, stream);
         if (rc != cudaSuccess) return static_cast<int>(rc);
       }
     }
@@ -1223,10 +1237,12 @@ int LaunchMatMulBiasAct(int dtype, const void* a, int64_t lda, bool transpose_a,
 }
 
 size_t MatMulGradWorkspaceBytes(const void* dy, const void* a, int64_t lda, bool transpose_a,
-                                const void* b, int64_t ldb, bool transpose_b, int64_t m,
-                                int64_t n, int64_t k, int act) {
+                                const void* b, int64_t ldb, bool transpose_b,
+                                const void* preactivation, int64_t m, int64_t n, int64_t k,
+                                int act) {
   if (BadSizes(m, n, k)) return 0;
-  return PlanGrad(dy, Factor{a, lda, transpose_a}, Factor{b, ldb, !transpose_b}, m, n, k, act)
+  return PlanGrad(dy, act == MUSA_ACT_IDENTITY ? nullptr : preactivation,
+                  Factor{a, lda, transpose_a}, Factor{b, ldb, !transpose_b}, m, n, k, act)
       .Total();
 }
 

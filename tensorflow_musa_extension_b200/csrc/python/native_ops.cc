@@ -666,7 +666,8 @@ PyObject* MatMulBiasActGrad(PyObject*, PyObject* const* o, Py_ssize_t count) {
   int rc;
   {
     const Scratch ws(g_api.MatMulGradWorkspaceBytes(dy->data_ptr(), a.data_ptr(), s.lda, ta,
-                                                    b.data_ptr(), s.ldb, tb, s.m, s.n, s.k, act));
+                                                    b.data_ptr(), s.ldb, tb, Data(z), s.m, s.n, s.k,
+                                                    act));
     pybind11::gil_scoped_release nogil;
     rc = g_api.LaunchMatMulBiasActGrad(DtypeCode(dtype), dy->data_ptr(), a.data_ptr(), s.lda, ta,
                                        b.data_ptr(), s.ldb, tb, Data(z), da.data_ptr(),

@@ -183,8 +183,8 @@ def MusaMatMulBiasActGrad(dy, a, b, preactivation=None, activation="Identity",
         fa, fb = a2.contiguous(), bd.contiguous()
         factors = (_r._ptr(fa), a2.shape[1], bool(transpose_a), _r._ptr(fb), bd.shape[1],
                    bool(transpose_b))
-        ws = _r._scratch(lib.MatMulGradWorkspaceBytes(_r._ptr(d), *factors, m, n, k, act),
-                         ad.device)
+        ws = _r._scratch(lib.MatMulGradWorkspaceBytes(_r._ptr(d), *factors, _r._ptr(z), m, n, k,
+                                                      act), ad.device)
         rc = lib.LaunchMatMulBiasActGrad(
             _r._DT_CODE[ad.dtype], _r._ptr(d), *factors, _r._ptr(z), _r._ptr(da), _r._ptr(db),
             _r._ptr(dbias), m, n, k, act, _r._ptr(ws), ws.numel(), _r._stream())
