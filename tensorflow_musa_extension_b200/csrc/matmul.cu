@@ -12,6 +12,7 @@
 // address, is first copied to lines that do.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <math.h>
 
 #include "common.cuh"
 #include "matmul.h"
@@ -104,29 +105,45 @@ __device__ __forceinline__ void Activate(float (&v)[kN], int act) {
   }
 }
 
-// act'(z)
-__device__ __forceinline__ float2 Slope(float2 z, int act) {
+// act'(z) in place of z.
+template <int kN>
+__device__ __forceinline__ void Slopes(float2 (&z)[kN], int act) {
   const float2 one = make_float2(1.0f, 1.0f);
   switch (act) {
     case MUSA_ACT_RELU:
-      return make_float2(z.x > 0.0f ? 1.0f : 0.0f, z.y > 0.0f ? 1.0f : 0.0f);
-    case MUSA_ACT_SIGMOID: {
-      const float2 p = SigmoidOf(z);
-      return Mul2(p, Add2(one, Neg2(p)));
-    }
-    case MUSA_ACT_SILU: {
-      const float2 p = SigmoidOf(z);
-      return Mul2(p, Fma2(z, Add2(one, Neg2(p)), one));
-    }
-    case MUSA_ACT_GELU: {
-      float2 bell;
-      const float2 tail = NormalTail(z, &bell);
-      const float2 phi = make_float2(z.x < 0.0f ? tail.x : 1.0f - tail.x,
-                                     z.y < 0.0f ? tail.y : 1.0f - tail.y);
-      return Fma2(Mul2(z, make_float2(0.39894228f, 0.39894228f)), bell, phi);
-    }
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        z[i] = make_float2(z[i].x > 0.0f ? 1.0f : 0.0f, z[i].y > 0.0f ? 1.0f : 0.0f);
+      }
+      break;
+    case MUSA_ACT_SIGMOID:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const float2 p = SigmoidOf(z[i]);
+        z[i] = Mul2(p, Add2(one, Neg2(p)));
+      }
+      break;
+    case MUSA_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const float2 p = SigmoidOf(z[i]);
+        z[i] = Mul2(p, Fma2(z[i], Add2(one, Neg2(p)), one));
+      }
+      break;
+    case MUSA_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        float2 bell;
+        const float2 tail = NormalTail(z[i], &bell);
+        const float2 phi = make_float2(z[i].x < 0.0f ? tail.x : 1.0f - tail.x,
+                                       z[i].y < 0.0f ? tail.y : 1.0f - tail.y);
+        z[i] = Fma2(Mul2(z[i], make_float2(0.39894228f, 0.39894228f)), bell, phi);
+      }
+      break;
     default:
-      return one;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) z[i] = one;
+      break;
   }
 }
 
@@ -164,32 +181,36 @@ __device__ __forceinline__ float LoadClusterF32At(uint32_t addr) {
   return v;
 }
 
-// Rows row .. row + kN - 1 of the product in column `col`: one value per lane and row.
-template <typename T, int kN>
-__device__ __forceinline__ void FinishColumn(float (&v)[kN], int64_t row, int64_t col,
+// What the epilogue of rows row .. row + kN - 1 of column `col` reads: asked for ahead of the
+// product, or of the chunk before.
+template <typename T, int kN, bool kBytes>
+struct ColumnInputs {
+  float residual[kN], scale[kBytes ? kN : 1];
+  __device__ __forceinline__ void Load(const SplitArgs& a, int64_t row, int rows, int64_t col) {
+    const T* at = static_cast<const T*>(a.e.residual) + row * a.n + col;
+    const bool add = a.e.residual != nullptr && col < a.n;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      residual[i] = add && i < rows ? ToF32(at[i * a.n]) : 0.0f;
+      if constexpr (kBytes) scale[i] = i < rows ? a.e.a_scale[row + i] : 0.0f;
+    }
+  }
+};
+
+// The first `rows` of rows row .. row + kN - 1 of the product in column `col`: one value per
+// lane and row.
+template <typename T, int kN, bool kBytes>
+__device__ __forceinline__ void FinishColumn(float (&v)[kN], const ColumnInputs<T, kN, kBytes>& in,
+                                             int64_t row, int rows, int64_t col,
                                              const SplitArgs& a, float bias, float col_scale) {
   const Epilogue& e = a.e;
   const bool inside = col < a.n;
   T* y = static_cast<T*>(e.y) + row * a.n + col;
-  const int rows = a.m - row < kN ? static_cast<int>(a.m - row) : kN;
-  float r[kN];
 #pragma unroll
-  for (int i = 0; i < kN; ++i) r[i] = 0.0f;
-  if (e.residual != nullptr) {
-    const T* at = static_cast<const T*>(e.residual) + row * a.n + col;
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      if (inside && i < rows) r[i] = ToF32(at[i * a.n]);
-    }
+  for (int i = 0; i < kN; ++i) {
+    if constexpr (kBytes) v[i] *= in.scale[i] * col_scale;
+    v[i] += bias;
   }
-  if (e.a_scale != nullptr) {
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      if (i < rows) v[i] *= e.a_scale[row + i] * col_scale;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kN; ++i) v[i] += bias;
   if (e.z != nullptr) {
     T* z = static_cast<T*>(e.z) + row * a.n + col;
 #pragma unroll
@@ -200,7 +221,7 @@ __device__ __forceinline__ void FinishColumn(float (&v)[kN], int64_t row, int64_
   Activate(v, e.act);
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
-    if (inside && i < rows) y[i * a.n] = FromF32<T>(v[i] + r[i]);
+    if (inside && i < rows) y[i * a.n] = FromF32<T>(v[i] + in.residual[i]);
   }
 }
 
@@ -299,32 +320,26 @@ __global__ void __launch_bounds__(kSplitThreads)
     if (ok && ElectLane()) MmaCommit<1>(SmemAddr(&done));
   }
   __syncwarp();
-  if (warp < 4 && last > first) {
-    ok = BarWait(SmemAddr(&done), 0, &give_up, &g_status);
-    TmemFenceAfter();
-  }
+  // This CTA's rows of the tile, in chunks: all of it, or its share of the cluster's.
+  constexpr int kChunkRows = 16;
+  const int share = a.rows_tile / a.splits;
+  const int64_t my_row = row0 + rank * share;
+  const int64_t left = a.m - my_row;
+  const int rows = warp >= 4 || left <= 0 ? 0 : left < share ? static_cast<int>(left) : share;
   const int64_t col = col0 + warp * 32 + lane;
   float bias = 0.0f, col_scale = 1.0f;
   if (warp < 4 && col < a.n) {
     if (a.e.bias != nullptr) bias = ToF32(static_cast<const T*>(a.e.bias)[col]);
-    if (a.e.b_scale != nullptr) col_scale = a.e.b_scale[col];
+    if (kBytes) col_scale = a.e.b_scale[col];
+  }
+  ColumnInputs<T, kChunkRows, kBytes> in;
+  in.Load(a, my_row, rows, col);
+  if (warp < 4 && last > first) {
+    ok = BarWait(SmemAddr(&done), 0, &give_up, &g_status);
+    TmemFenceAfter();
   }
   const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
-  if (a.splits == 1) {
-    if (warp < 4 && ok) {
-      for (int c = 0; c < a.rows_tile && row0 + c < a.m; c += 16) {
-        float v[16];
-        if (last > first) {
-          TmemLoad(lanes + c, v);
-          TmemLoadWait(v);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-        }
-        FinishColumn<T>(v, row0 + c, col, a, bias, col_scale);
-      }
-    }
-  } else {
+  if (a.splits > 1) {
     // Partial tile [row][128 columns] over the ring: this CTA's copies and matrix
     // instructions are done.
     if (warp < 4 && ok) {
@@ -341,21 +356,35 @@ __global__ void __launch_bounds__(kSplitThreads)
       }
     }
     ClusterSync();
-    if (warp < 4 && ok) {
-      const int share = a.rows_tile / a.splits;
-      for (int c = 0; c < share; c += 2) {
-        const int row = static_cast<int>(rank) * share + c;
-        float v[2] = {0.0f, 0.0f};
-        for (int s = 0; s < a.splits; ++s) {
-          const uint32_t at = MapToCta(ring + (row * 128 + warp * 32 + lane) * 4, s);
-          v[0] += LoadClusterF32At(at);
-          v[1] += LoadClusterF32At(at + 512);
-        }
-        if (row0 + row < a.m) FinishColumn<T>(v, row0 + row, col, a, bias, col_scale);
-      }
-    }
-    ClusterSync();
   }
+  if (ok) {
+    for (int c = 0; c < rows; c += kChunkRows) {
+      float v[kChunkRows];
+#pragma unroll
+      for (int i = 0; i < kChunkRows; ++i) v[i] = 0.0f;
+      if (a.splits > 1) {
+        // In rank order.  Rows of the chunk behind the share are not asked for.
+        const uint32_t mine =
+            ring + ((static_cast<int>(rank) * share + c) * 128 + warp * 32 + lane) * 4;
+#pragma unroll 2
+        for (int s = 0; s < a.splits; ++s) {
+          const uint32_t at = MapToCta(mine, s);
+#pragma unroll
+          for (int i = 0; i < kChunkRows; ++i) {
+            if (c + i < rows) v[i] += LoadClusterF32At(at + i * 512);
+          }
+        }
+      } else if (last > first) {
+        TmemLoad(lanes + c, v);
+        TmemLoadWait(v);
+      }
+      const ColumnInputs<T, kChunkRows, kBytes> now = in;
+      const int next = c + kChunkRows;
+      if (next < rows) in.Load(a, my_row + next, rows - next, col);
+      FinishColumn<T>(v, now, my_row + c, rows - c, col, a, bias, col_scale);
+    }
+  }
+  if (a.splits > 1) ClusterSync();
   TmemFenceBefore();
   __syncthreads();
   if (give_up != 0) LeaveInFlight();
@@ -438,22 +467,37 @@ __device__ __forceinline__ void StorePiece(uint32_t at, const float* v) {
 }
 
 // A tile of up to 128 x kChunk elements between global memory and swizzled shared memory, by
-// the 128 threads of a group.
+// the 128 threads of a group: a warp a line, sixteen lines in flight (one after the other, the
+// residual of a 333 x 2047 product took as long as the rest of it).
 template <typename T, bool kToShared>
 __device__ __forceinline__ void MoveTile(uint32_t tile, T* global, int64_t row0, int64_t col0,
                                          const PairArgs& a, int thread) {
-  for (int i = thread; i < 128 * kChunk; i += 128) {
-    const int line = i / kChunk, c = i % kChunk;
-    const uint32_t at = Swizzled(tile, line, c >> 3) + (c & 7) * 2;
-    if (row0 + line < a.m && col0 + c < a.n) {
-      T* g = global + (row0 + line) * a.n + col0 + c;
+  static_assert(kChunk == 32, "a lane per column");
+  constexpr int kBatch = 16;
+  const int c = thread % 32;
+  const int64_t left = col0 + c < a.n ? a.m - row0 : 0;
+  T* at = global + row0 * a.n + col0 + c;
+  const auto Shared = [&](int line) { return Swizzled(tile, line, c >> 3) + (c & 7) * 2; };
+  for (int first = thread / 32; first < 128; first += 4 * kBatch) {
+    uint16_t v[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int line = first + 4 * i;
       if constexpr (kToShared) {
-        const uint16_t v = *reinterpret_cast<const uint16_t*>(g);
-        asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
+        if (line < left) v[i] = *reinterpret_cast<const uint16_t*>(at + line * a.n);
       } else {
-        uint16_t v;
-        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
-        *reinterpret_cast<uint16_t*>(g) = v;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v[i]) : "r"(Shared(line)) : "memory");
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int line = first + 4 * i;
+      if (line < left) {
+        if constexpr (kToShared) {
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(Shared(line)), "h"(v[i]) : "memory");
+        } else {
+          *reinterpret_cast<uint16_t*>(at + line * a.n) = v[i];
+        }
       }
     }
   }
@@ -826,9 +870,15 @@ bool MakeMap(CUtensorMap* map, const void* p, int64_t count, int64_t length, int
 
 // ---------------------------------------------------------------- launches --
 
+constexpr int kSplitSmem = 208 * 1024;  // for the stages of an SM's CTAs
+
+int SplitCtasPerSm(int rows_tile) {
+  return (kSideBytes + rows_tile * kDepthBytes) * 4 <= kSplitSmem / 2 ? 2 : 1;
+}
+
 template <typename T, bool kBytes>
 int LaunchSplit(int64_t m, int64_t n, int64_t k, const Factor& fa, const Factor& fb,
-                const Epilogue& e, cudaStream_t stream) {
+                const Epilogue& e, int rows_tile, int splits, cudaStream_t stream) {
   using E = std::conditional_t<kBytes, uint8_t, T>;
   constexpr int kDepth = 128 / sizeof(E);
   SplitArgs a = {};
@@ -838,18 +888,17 @@ int LaunchSplit(int64_t m, int64_t n, int64_t k, const Factor& fa, const Factor&
   a.blocks = static_cast<int>(CeilDiv(k, kDepth));
   a.p_rows = fb.rows_contiguous;
   a.q_rows = fa.rows_contiguous;
-  a.rows_tile = static_cast<int>(m >= 256 ? 256 : RoundUp(m, a.q_rows ? 64 : 16));
+  a.rows_tile = rows_tile;
+  a.splits = splits;
   a.stage_bytes = kSideBytes + a.rows_tile * kDepthBytes;
-  // Two CTAs per SM where four stages fit half an SM's shared memory.
-  const int budget = a.stage_bytes * 4 <= 104 * 1024 ? 104 * 1024 : 208 * 1024;
+  // Copies in flight carry a CTA through its depth: all the shared memory where it has an SM
+  // to itself, half where four stages fit that.  Clusters of eight that need eight whole SMs
+  // each do not fill the machine (128 such CTAs took 20 us where 128 of half an SM took 12).
+  const int64_t ctas = CeilDiv(n, 128) * CeilDiv(m, rows_tile) * splits;
+  const bool whole = SplitCtasPerSm(rows_tile) == 1 || ctas <= SmCount() / (splits == 8 ? 2 : 1);
+  const int budget = whole ? kSplitSmem : kSplitSmem / 2;
   a.stages = budget / a.stage_bytes;
   if (a.stages > kMaxStages) a.stages = kMaxStages;
-  const int64_t tiles = CeilDiv(n, 128) * CeilDiv(m, a.rows_tile);
-  const int64_t slots = static_cast<int64_t>(SmCount()) * (budget < 128 * 1024 ? 2 : 1);
-  a.splits = 1;
-  while (a.splits < 8 && tiles * a.splits * 2 <= slots && a.blocks >= a.splits * 2 * 2) {
-    a.splits *= 2;
-  }
   a.tmem_columns = 32;
   while (a.tmem_columns < static_cast<uint32_t>(a.rows_tile)) a.tmem_columns *= 2;
   constexpr int kType = kBytes ? 0 : std::is_same_v<T, __nv_bfloat16> ? 1 : 0;
@@ -962,24 +1011,101 @@ int LaunchPair(int64_t m, int64_t n, int64_t k, const Factor& fa, const Factor& 
                                              maps[2], maps[3], maps[4], a));
 }
 
-// Which form: pairs where their tiles come near to filling the machine, columns of 128
-// where those of 256 leave it a third empty; the split form below that.
+// The form of a product.
+struct Plan {
+  int tile_n;             // pairs with tiles of this many columns, or 0: the split form
+  int rows_tile, splits;  // of the split form
+};
+
+// The form whose estimated time is least.  An estimate adds up what bounds a form, at rates
+// taken from a sweep of every form over 160 sizes (1 .. 2000 rows, both factor types): the
+// longest of the depth steps of the waves of CTAs one after the other, the factors' copies
+// out of L2 and the reads of HBM; then the epilogues of the waves, which a split tile pays with
+// the exchange of its partial sums.  Over that sweep the choice was 5% off the best form in
+// the mean; fixed tiles of 256 rows were 35% off (1000 x 640, depth 1408: 19.2 us against 8.9;
+// 256 x 1000, depth 520: 15.7 against 6.6; one row x 4096, depth 4096: 12.1 against 11.0).
+constexpr double kMbPerUs = 1e-6;
+
+// Near-equal bounds of one stretch add a little to the longest.
+double Longest(double a, double b, double c, double d) {
+  const auto Fourth = [](double v) { return v * v * v * v; };
+  return sqrt(sqrt(Fourth(a) + Fourth(b) + Fourth(c) + Fourth(d)));
+}
+
+double SplitMicroseconds(int64_t m, int64_t n, int blocks, double hbm_bytes, int rows_tile,
+                         int splits) {
+  const int per_sm = SplitCtasPerSm(rows_tile);
+  const int64_t ctas = CeilDiv(n, 128) * CeilDiv(m, rows_tile) * splits;
+  // Clusters of eight fit the SMs' groups 14 times.
+  const int64_t waves = CeilDiv(ctas, (splits == 8 ? 112 : SmCount()) * per_sm);
+  const int64_t steps = CeilDiv(blocks, splits);
+  const double copied = static_cast<double>(ctas) * steps * (kSideBytes + rows_tile * kDepthBytes);
+  const double rows = rows_tile * (per_sm == 2 && ctas > SmCount() ? 2.0 : 1.0);
+  double epilogue = 0.0704 * rows / splits;
+  if (splits > 1) epilogue += 0.0142 * rows + 1.82 + 0.327 * splits;
+  return 1.94 + Longest(waves * steps * 0.194, waves * steps * rows * 0.0014,
+                        copied * kMbPerUs / 18.2, hbm_bytes * kMbPerUs / 6.47) +
+         waves * epilogue;
+}
+
+double PairMicroseconds(int64_t m, int64_t n, int blocks, double hbm_bytes, int tile_n) {
+  const int64_t tiles = CeilDiv(m, 256) * CeilDiv(n, tile_n);
+  const int64_t rounds = CeilDiv(tiles, SmCount() / 2);
+  const double copied = static_cast<double>(tiles) * blocks * (256 + tile_n) * kDepthBytes;
+  // Outputs that TMA cannot address go element by element (333 x 2047 with all outputs: 21 us,
+  // 333 x 2048 11).
+  const double moves = n % 8 != 0 ? 3.0 * tile_n / 128 : 0.0;
+  return 4.87 + Longest(rounds * blocks * (tile_n == 256 ? 0.311 : 0.201), 0.0,
+                        copied * kMbPerUs / 18.0, hbm_bytes * kMbPerUs / 5.83) +
+         rounds * ((tile_n == 256 ? 2.17 : 1.17) + moves);
+}
+
+// The choice does not depend on how the factors are stored: it decides the order of the sums.
+Plan PlanProduct(int64_t m, int64_t n, int blocks, bool a_rows) {
+  const int form = GetTuning(kTuneMatMulForm);
+  const int64_t most = RoundUp(m, 16);
+  const auto Tile = [most](int64_t rows) { return static_cast<int>(rows < most ? rows : most); };
+  Plan best = {0, Tile(256), 1};
+  if (form >= 16) {
+    best.rows_tile = Tile(form & ~15);
+    best.splits = form & 15;
+  } else if (blocks > 0 && (form == 2 || form == 3)) {
+    best.tile_n = form == 2 ? 256 : 128;
+  } else if (blocks > 0) {
+    const double hbm_bytes = (static_cast<double>(m) + n) * blocks * kDepthBytes + 4.0 * m * n;
+    double least = 1e300;
+    for (int rows = 16; rows <= 256; rows *= 2) {
+      for (int splits = 1; splits <= 8 && splits <= blocks; splits *= 2) {
+        const double t = SplitMicroseconds(m, n, blocks, hbm_bytes, Tile(rows), splits);
+        if (t < least) {
+          least = t;
+          best.rows_tile = Tile(rows);
+          best.splits = splits;
+        }
+      }
+      if (rows >= most) break;
+    }
+    for (int tile_n = 128; tile_n <= 256 && form == 0; tile_n *= 2) {
+      const double t = PairMicroseconds(m, n, blocks, hbm_bytes, tile_n);
+      if (t < least) {
+        least = t;
+        best.tile_n = tile_n;
+      }
+    }
+  }
+  // Blocks of 64 rows where they are contiguous.
+  if (a_rows) best.rows_tile = static_cast<int>(RoundUp(best.rows_tile, 64));
+  return best;
+}
+
 template <typename T, bool kBytes>
 int Product(int64_t m, int64_t n, int64_t k, const Factor& fa, const Factor& fb,
             const Epilogue& e, cudaStream_t stream) {
-  const int form = GetTuning(kTuneMatMulForm);
-  int tile_n = 0;
-  if (form == 0) {
-    const int64_t pairs = SmCount() / 2;
-    const int64_t wide = CeilDiv(m, 256) * CeilDiv(n, 256);
-    const int64_t narrow = CeilDiv(m, 256) * CeilDiv(n, 128);
-    if (m > 128 && k > 0 && wide * 3 >= pairs * 2) tile_n = 256;
-    else if (m > 128 && k > 0 && narrow * 3 >= pairs * 2) tile_n = 128;
-  } else if (form >= 2 && k > 0) {
-    tile_n = form == 2 ? 256 : 128;
-  }
-  if (tile_n != 0) return LaunchPair<T, kBytes>(m, n, k, fa, fb, e, tile_n, stream);
-  return LaunchSplit<T, kBytes>(m, n, k, fa, fb, e, stream);
+  const int blocks = static_cast<int>(CeilDiv(k * static_cast<int64_t>(kBytes ? 1 : sizeof(T)), 128));
+  const Plan p = PlanProduct(m, n, blocks, fa.rows_contiguous);
+  return p.tile_n != 0
+             ? LaunchPair<T, kBytes>(m, n, k, fa, fb, e, p.tile_n, stream)
+             : LaunchSplit<T, kBytes>(m, n, k, fa, fb, e, p.rows_tile, p.splits, stream);
 }
 
 // ---------------------------------------------------------------- gradient --
@@ -999,12 +1125,20 @@ struct SlopeArgs {
   int act;
 };
 
-constexpr int kSumCtas = 3;      // per SM: one wave of them, 85 registers
+constexpr int kSumCtas = 2;      // per SM: one wave of them, 128 registers
 
 template <typename T, int kVec>
 __global__ void __launch_bounds__(32 * kSumRows, kSumCtas) SlopeKernel(SlopeArgs a) {
   using P = Pack<T, kVec>;
-  constexpr int kUnroll = 4;
+  constexpr int kUnroll = 4, kPairs = (kVec + 1) / 2;
+  const auto Widen = [](const P& p, float2 (&v)[kPairs]) {
+    if constexpr (kVec == 1) v[0] = make_float2(ToF32(p.v[0]), 0.0f);
+    else WidenPack<kVec>(p, v);
+  };
+  const auto Narrow = [](const float2 (&v)[kPairs], P& p) {
+    if constexpr (kVec == 1) p.v[0] = FromF32<T>(v[0].x);
+    else NarrowPack<kVec>(v, p);
+  };
   __shared__ float sums[kSumRows][32 * kVec + 1];
   GridDepWait();
   GridDepLaunch();
@@ -1013,9 +1147,9 @@ __global__ void __launch_bounds__(32 * kSumRows, kSumCtas) SlopeKernel(SlopeArgs
   const int64_t begin = blockIdx.y * a.rows_per_cta;
   const int64_t end = begin + a.rows_per_cta < a.m ? begin + a.rows_per_cta : a.m;
   const bool bent = a.act != MUSA_ACT_IDENTITY;
-  float sum[kVec];
+  float2 sum[kPairs];
 #pragma unroll
-  for (int e = 0; e < kVec; ++e) sum[e] = 0.0f;
+  for (int e = 0; e < kPairs; ++e) sum[e] = make_float2(0.0f, 0.0f);
   if (col < a.n) {
     const T* dy = static_cast<const T*>(a.dy) + col;
     const T* z = static_cast<const T*>(a.z) + col;
@@ -1034,30 +1168,26 @@ __global__ void __launch_bounds__(32 * kSumRows, kSumCtas) SlopeKernel(SlopeArgs
       for (int u = 0; u < kUnroll; ++u) {
         const int64_t row = r + u * kSumRows;
         if (row >= end) break;
+        float2 d[kPairs];
+        Widen(g[u], d);
         if (bent) {
+          float2 slope[kPairs];
+          Widen(x[u], slope);
+          Slopes(slope, a.act);
 #pragma unroll
-          for (int e = 0; e < kVec; e += 2) {
-            const int f = kVec > 1 ? e + 1 : e;
-            const float2 slope = Slope(make_float2(ToF32(x[u].v[e]), ToF32(x[u].v[f])), a.act);
-            const float d0 = ToF32(g[u].v[e]) * slope.x;
-            sum[e] += d0;
-            g[u].v[e] = FromF32<T>(d0);
-            if (kVec > 1) {
-              const float d1 = ToF32(g[u].v[f]) * slope.y;
-              sum[f] += d1;
-              g[u].v[f] = FromF32<T>(d1);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) sum[e] += ToF32(g[u].v[e]);
+          for (int e = 0; e < kPairs; ++e) d[e] = Mul2(d[e], slope[e]);
+          Narrow(d, g[u]);
         }
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) sum[e] = Add2(sum[e], d[e]);
         if (a.dz != nullptr) *reinterpret_cast<P*>(dz + row * a.pitch) = g[u];
       }
     }
   }
 #pragma unroll
-  for (int e = 0; e < kVec; ++e) sums[row_lane][lane * kVec + e] = sum[e];
+  for (int e = 0; e < kVec; ++e) {
+    sums[row_lane][lane * kVec + e] = e % 2 == 0 ? sum[e / 2].x : sum[e / 2].y;
+  }
   __syncthreads();
   for (int c = threadIdx.x; c < 32 * kVec; c += 32 * kSumRows) {
     const int64_t at = static_cast<int64_t>(blockIdx.x) * 32 * kVec + c;

@@ -42,7 +42,8 @@ enum TuningKey {
   kTuneBnGridRefuse = 28,   // 1: the grid-wide form's launch answers that it is too large for the context
                             // (what the caller does then is tested with it)
   kTuneMatMulForm = 29,     // form of the matrix products: 0 by rule, 1 split, 2 and 3 pairs of CTAs with
-                            // tiles of 256 and 128 columns
+                            // tiles of 256 and 128 columns, 16 or more the split form with row
+                            // tiles of `value & ~15` rows and `value & 15` CTAs a tile
   kTuneCount = 30
 };
 
