@@ -61,12 +61,12 @@ __device__ __forceinline__ void GroupSumMax(float& v, unsigned& w, int group, fl
       if (kMax) tops[warp] = w;
     }
     __syncthreads();
-    v = 0.0f;
-    w = 0;
-    for (int i = 0; i < warps; ++i) {
-      v += sums[first + i];
-      if (kMax) w = max(w, tops[first + i]);
-    }
+    // Each warp folds the warps' values (every lane reading all of them was a third of the
+    // instructions of a row of 8192).
+    const int from = first + (threadIdx.x & (warps - 1));
+    v = sums[from];
+    if (kMax) w = __reduce_max_sync(0xffffffffu, tops[from]);
+    for (int m = warps / 2; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
   }
 }
 
@@ -80,10 +80,10 @@ __device__ __forceinline__ float QuantizeScale(float top) {
   return t < kScaleMin ? kScaleMin : t;  // NaN goes through
 }
 
-// The larger of `w` and |v|; NaN stays.
-__device__ __forceinline__ float MaxMagnitude(float w, float v) {
+// The largest magnitude of `w` and the pair; NaN stays.
+__device__ __forceinline__ float MaxMagnitude(float w, float2 v) {
   float out;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(out) : "f"(w), "f"(fabsf(v)));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(out) : "f"(w), "f"(v.x), "f"(v.y));
   return out;
 }
 
@@ -218,31 +218,46 @@ __global__ void __launch_bounds__(1024) AddNormKernel(AddNormArgs a) {
   int64_t row = base + threadIdx.x / a.group;
   RowView<T, kShifted> view(row, a.rows, a.row_size);
   const int64_t jump = step * a.row_size;
-  const auto Widen = [](const uint4* slot, float2 (&v)[kVec / 2]) {
-    const uint4 w = *slot;
+  const auto Widen = [](const char* slot, float2 (&v)[kVec / 2]) {
+    const uint4 w = *reinterpret_cast<const uint4*>(slot);
     WidenPack<kVec>(*reinterpret_cast<const P*>(&w), v);
   };
-  const auto Slot = [&](int stage, int input, int j) {
-    return ring + ((stage * 2 + input) * kPacks + j) * blockDim.x + threadIdx.x;
-  };
-  // Packs of the row `ahead` rounds on to a stage; one group of copies, maybe empty.
-  const auto Ask = [&](int stage, int ahead) {
-    if (row + ahead * step < a.rows) {
-      RowView<T, kShifted> at = view;
-      at.first += ahead * jump;
+  // Slots of this thread: pack j of input i of a stage lies (i * kPacks + j) * pitch behind it.
+  const int pitch = blockDim.x * 16, stage_bytes = 2 * kPacks * pitch;
+  char* slots = reinterpret_cast<char*>(ring + threadIdx.x);
+  // Where the next row to ask for lies; its packs are `hop` elements apart.
+  const int hop = a.group * kVec;
+  const T* next_x = static_cast<const T*>(a.x) + view.first + t * kVec;
+  const T* next_r = add ? static_cast<const T*>(a.residual) + view.first + t * kVec : nullptr;
+  int64_t next_row = row;
+  // The tensor's last pack: what lies behind it is not read and comes as zeros.
+  const int tail = view.row_size + view.shift - (view.packs - 1) * kVec;
+  // One group of copies, maybe empty.
+  const auto Ask = [&](char* stage) {
+    if (next_row < a.rows) {
 #pragma unroll
       for (int j = 0; j < kPacks; ++j) {
         const int p = t + j * a.group;
         if (p < view.packs) {
-          at.Copy(Slot(stage, 0, j), a.x, p);
-          if (add) at.Copy(Slot(stage, 1, j), a.residual, p);
+          uint4* x_slot = reinterpret_cast<uint4*>(stage + j * pitch);
+          uint4* r_slot = reinterpret_cast<uint4*>(stage + (kPacks + j) * pitch);
+          if (kShifted && next_row == a.rows - 1 && p == view.packs - 1) {
+            CopyPart(x_slot, next_x + j * hop, tail * static_cast<int>(sizeof(T)));
+            if (add) CopyPart(r_slot, next_r + j * hop, tail * static_cast<int>(sizeof(T)));
+          } else {
+            CopyPack(x_slot, next_x + j * hop);
+            if (add) CopyPack(r_slot, next_r + j * hop);
+          }
         }
       }
     }
     CopyCommit();
+    next_row += step;
+    next_x += jump;
+    next_r += jump;
   };
 #pragma unroll
-  for (int i = 0; i < kStages; ++i) Ask(i, i);
+  for (int i = 0; i < kStages; ++i) Ask(slots + i * stage_bytes);
   P gamma[kPacks];
 #pragma unroll
   for (int j = 0; j < kPacks; ++j) {
@@ -254,6 +269,8 @@ __global__ void __launch_bounds__(1024) AddNormKernel(AddNormArgs a) {
   for (int64_t at = base; at < a.rows; at += step) {
     const bool there = row < a.rows;
     CopyWait<kStages - 1>();
+    char* slot = slots + stage * stage_bytes;
+    // s, then s * gamma: `sum` is written before the reduction.
     float2 s[kPacks][kVec / 2];
     float2 squares = make_float2(0.0f, 0.0f);
     float largest = 0.0f;
@@ -261,45 +278,16 @@ __global__ void __launch_bounds__(1024) AddNormKernel(AddNormArgs a) {
     for (int j = 0; j < kPacks; ++j) {
       const int p = t + j * a.group;
       if (there && p < view.packs) {
-        Widen(Slot(stage, 0, j), s[j]);
+        Widen(slot + j * pitch, s[j]);
         if (add) {
           float2 r[kVec / 2];
-          Widen(Slot(stage, 1, j), r);
+          Widen(slot + (kPacks + j) * pitch, r);
 #pragma unroll
           for (int e = 0; e < kVec / 2; ++e) s[j][e] = Add2(s[j][e], r[e]);
         }
         view.Mask(p, s[j]);
-        float2 g[kVec / 2];
-        if (kQuantize && normed) WidenPack<kVec>(gamma[j], g);
 #pragma unroll
-        for (int e = 0; e < kVec / 2; ++e) {
-          squares = Fma2(s[j][e], s[j][e], squares);
-          if constexpr (kQuantize) {
-            const float2 v = normed ? Mul2(s[j][e], g[e]) : s[j][e];
-            largest = MaxMagnitude(MaxMagnitude(largest, v.x), v.y);
-          }
-        }
-      }
-    }
-    Ask(stage, kStages);
-    if (++stage == kStages) stage = 0;
-    float square = squares.x + squares.y;
-    unsigned top = MagnitudeBits(largest);
-    GroupSumMax<kQuantize>(square, top, a.group, sums[parity], tops[parity]);
-    parity ^= 1;
-    float inv = rsqrtf(fmaf(square, a.inv_size, a.epsilon));
-    if (!normed) inv = 1.0f;
-    float scale = 1.0f, unscale = 1.0f;
-    if constexpr (kQuantize) {
-      scale = QuantizeScale(__uint_as_float(top) * inv);
-      unscale = 1.0f / scale;
-    }
-    if (there && t == 0) a.stat[row] = kQuantize ? scale : inv;
-    const float2 invs = make_float2(inv, inv), unscales = make_float2(unscale, unscale);
-#pragma unroll
-    for (int j = 0; j < kPacks; ++j) {
-      const int p = t + j * a.group;
-      if (there && p < view.packs) {
+        for (int e = 0; e < kVec / 2; ++e) squares = Fma2(s[j][e], s[j][e], squares);
         if (!kQuantize || a.sum != nullptr) {
           P total;
           NarrowPack<kVec>(s[j], total);
@@ -309,15 +297,49 @@ __global__ void __launch_bounds__(1024) AddNormKernel(AddNormArgs a) {
           float2 g[kVec / 2];
           WidenPack<kVec>(gamma[j], g);
 #pragma unroll
-          for (int e = 0; e < kVec / 2; ++e) {
-            s[j][e] = Mul2(Mul2(s[j][e], invs), g[e]);
-            // Last: inv / scale alone passes the largest float in a row of zeros.
-            if (kQuantize) s[j][e] = Mul2(s[j][e], unscales);
+          for (int e = 0; e < kVec / 2; ++e) s[j][e] = Mul2(s[j][e], g[e]);
+        }
+        if constexpr (kQuantize) {
+#pragma unroll
+          for (int e = 0; e < kVec / 2; ++e) largest = MaxMagnitude(largest, s[j][e]);
+        }
+      }
+    }
+    Ask(slot);
+    if (++stage == kStages) stage = 0;
+    float square = squares.x + squares.y;
+    unsigned top = MagnitudeBits(largest);
+    GroupSumMax<kQuantize>(square, top, a.group, sums[parity], tops[parity]);
+    parity ^= 1;
+    float inv = rsqrtf(fmaf(square, a.inv_size, a.epsilon));
+    if (!normed) inv = 1.0f;
+    float scale = 1.0f, factor = inv, second = 1.0f;
+    if constexpr (kQuantize) {
+      scale = QuantizeScale(__uint_as_float(top) * inv);
+      factor = inv / scale;
+      // It passes the largest float in rows of values near zero: one after the other there.
+      if (!(factor < 3.4e38f)) {
+        factor = inv;
+        second = 1.0f / scale;
+      }
+    }
+    if (there && t == 0) a.stat[row] = kQuantize ? scale : inv;
+    const float2 factors = make_float2(factor, factor), seconds = make_float2(second, second);
+#pragma unroll
+    for (int j = 0; j < kPacks; ++j) {
+      const int p = t + j * a.group;
+      if (there && p < view.packs) {
+        if (normed) {
+#pragma unroll
+          for (int e = 0; e < kVec / 2; ++e) s[j][e] = Mul2(s[j][e], factors);
+          if (kQuantize && second != 1.0f) {
+#pragma unroll
+            for (int e = 0; e < kVec / 2; ++e) s[j][e] = Mul2(s[j][e], seconds);
           }
         } else {
           // Rows as they are take the rounded division: quotients of 16-bit values fall on
           // borders between two e4m3 values, where a last bit decides.  Behind a norm the
-          // fp32 values are off by more than the product with the reciprocal.
+          // fp32 values are off by more than the product with the factor.
 #pragma unroll
           for (int e = 0; e < kVec / 2; ++e) {
             s[j][e] = make_float2(s[j][e].x / scale, s[j][e].y / scale);
