@@ -762,32 +762,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
 // ---------------------------------------------------------------- factors --
 
-// Lines of `columns` elements, `ld` apart, to lines `pitch` apart; up to two factors in one
-// launch, blockIdx.z one of them.
-struct RepitchArgs {
-  const void* src;
-  void* dst;
-  int64_t lines, columns, ld, pitch;
-};
-struct RepitchPair {
-  RepitchArgs of[2];
-};
-
+// Lines of `columns` elements, `ld` apart, to lines `pitch` apart.
 template <typename E>
-__global__ void __launch_bounds__(256) RepitchKernel(const __grid_constant__ RepitchPair pair) {
+__global__ void __launch_bounds__(256)
+    RepitchKernel(const E* __restrict__ src, E* __restrict__ dst, int64_t lines, int64_t columns,
+                  int64_t ld, int64_t pitch) {
   GridDepWait();
   GridDepLaunch();
-  const RepitchArgs a = pair.of[blockIdx.z];
-  const E* src = static_cast<const E*>(a.src);
-  E* dst = static_cast<E*>(a.dst);
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x;
-  if (c >= a.columns) return;
-  for (int64_t r = blockIdx.y; r < a.lines; r += gridDim.y) {
+  for (int64_t r = blockIdx.y; r < lines; r += gridDim.y) {
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (c + i * 256 < a.columns) {
-        dst[r * a.pitch + c + i * 256] = src[r * a.ld + c + i * 256];
-      }
+      if (c + i * 256 < columns) dst[r * pitch + c + i * 256] = src[r * ld + c + i * 256];
     }
   }
 }
@@ -814,32 +800,26 @@ size_t RepitchBytes(const Factor& f, int64_t rows, int64_t depth, int elem) {
   return static_cast<size_t>(RoundUp(l.length * elem, 16) * l.count + 16);
 }
 
-// Copies what TMA cannot address of op(a) [m, k] and op(b) [n, k] (null: not wanted) to the
-// workspace.
-cudaError_t Repitch(Factor* a, Factor* b, int64_t m, int64_t n, int64_t k, int elem,
-                    uint8_t* workspace, cudaStream_t stream) {
-  RepitchPair pair = {};
-  unsigned count = 0;
-  int64_t columns = 0, lines = 0;
-  for (const bool first : {true, false}) {
-    Factor* f = first ? a : b;
-    const int64_t rows = first ? m : n;
-    const size_t bytes = f != nullptr ? RepitchBytes(*f, rows, k, elem) : 0;
-    if (bytes == 0) continue;
-    const Lines l = LinesOf(*f, rows, k);
-    const int64_t pitch = RoundUp(l.length * elem, 16) / elem;
-    pair.of[count++] = {f->p, workspace, l.count, l.length, f->ld, pitch};
-    if (l.length > columns) columns = l.length;
-    if (l.count > lines) lines = l.count;
-    f->p = workspace;
-    f->ld = pitch;
-    workspace += RoundUp(static_cast<int64_t>(bytes), 16);
-  }
-  if (count == 0) return cudaSuccess;
-  const dim3 grid(static_cast<unsigned>(CeilDiv(columns, 1024)),
-                  static_cast<unsigned>(lines < 32768 ? lines : 32768), count);
-  return elem == 2 ? LaunchChained(true, RepitchKernel<uint16_t>, grid, dim3(256), 0, stream, pair)
-                   : LaunchChained(true, RepitchKernel<uint8_t>, grid, dim3(256), 0, stream, pair);
+cudaError_t Repitch(Factor* f, int64_t rows, int64_t depth, int elem, uint8_t** workspace,
+                    cudaStream_t stream) {
+  const size_t bytes = RepitchBytes(*f, rows, depth, elem);
+  if (bytes == 0) return cudaSuccess;
+  const Lines l = LinesOf(*f, rows, depth);
+  const int64_t pitch = RoundUp(l.length * elem, 16) / elem;
+  const dim3 grid(static_cast<unsigned>(CeilDiv(l.length, 1024)),
+                  static_cast<unsigned>(l.count < 32768 ? l.count : 32768));
+  const cudaError_t rc =
+      elem == 2 ? LaunchChained(true, RepitchKernel<uint16_t>, grid, dim3(256), 0, stream,
+                                static_cast<const uint16_t*>(f->p),
+                                reinterpret_cast<uint16_t*>(*workspace), l.count, l.length, f->ld,
+                                pitch)
+                : LaunchChained(true, RepitchKernel<uint8_t>, grid, dim3(256), 0, stream,
+                                static_cast<const uint8_t*>(f->p), *workspace, l.count, l.length,
+                                f->ld, pitch);
+  f->p = *workspace;
+  f->ld = pitch;
+  *workspace += RoundUp(static_cast<int64_t>(bytes), 16);
+  return rc;
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -1284,8 +1264,9 @@ int Forward(Factor a, Factor b, const Epilogue& e, int64_t m, int64_t n, int64_t
   if (BadWorkspace(workspace, bytes, RepitchBytes(a, m, k, 2) + RepitchBytes(b, n, k, 2))) {
     return MUSA_KERNELS_EWORKSPACE;
   }
-  const cudaError_t rc =
-      Repitch(&a, &b, m, n, k, 2, static_cast<uint8_t*>(workspace), stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  cudaError_t rc = Repitch(&a, m, k, 2, &ws, stream);
+  if (rc == cudaSuccess) rc = Repitch(&b, n, k, 2, &ws, stream);
   return rc != cudaSuccess ? static_cast<int>(rc)
                            : Product<T, false>(m, n, k, a, b, e, stream);
 }
@@ -1319,10 +1300,8 @@ int Backward(const void* dy, Factor a, Factor b, const void* z, void* da, void* 
     cudaMemsetAsync(dbias, 0, sizeof(T) * n, stream);
   }
   rc = cudaGetLastError();
-  if (rc == cudaSuccess) {
-    rc = Repitch(db != nullptr ? &a : nullptr, da != nullptr ? &b : nullptr, m, n, k, 2, ws,
-                 stream);
-  }
+  if (rc == cudaSuccess && db != nullptr && m > 0) rc = Repitch(&a, m, k, 2, &ws, stream);
+  if (rc == cudaSuccess && da != nullptr && n > 0) rc = Repitch(&b, n, k, 2, &ws, stream);
   if (rc != cudaSuccess) return static_cast<int>(rc);
   const void* g = p.want_dz ? dz : dy;
   const int64_t ldg = p.want_dz ? p.dz_pitch : n;
@@ -1442,8 +1421,9 @@ int LaunchQuantizedMatMulBiasAct(int out_dtype, const void* a, int64_t lda, cons
                    RepitchBytes(fa, m, k, 1) + RepitchBytes(fb, n, k, 1))) {
     return MUSA_KERNELS_EWORKSPACE;
   }
-  const cudaError_t rc =
-      Repitch(&fa, &fb, m, n, k, 1, static_cast<uint8_t*>(workspace), stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  cudaError_t rc = Repitch(&fa, m, k, 1, &ws, stream);
+  if (rc == cudaSuccess) rc = Repitch(&fb, n, k, 1, &ws, stream);
   if (rc != cudaSuccess) return static_cast<int>(rc);
   const Epilogue e = {bias, residual, a_scale, b_scale, y, nullptr, act};
   return out_dtype == MUSA_DT_F16 ? Product<__half, true>(m, n, k, fa, fb, e, stream)
