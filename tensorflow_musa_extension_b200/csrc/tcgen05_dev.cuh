@@ -122,10 +122,6 @@ __device__ __forceinline__ void TmaStoreWaitAll() {
 __device__ __forceinline__ void FenceAsyncShared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
-__device__ __forceinline__ void TmaPrefetch(const CUtensorMap* map) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-}
-
 // ---- Tensor memory: 128 lanes x 512 columns of 32 bits per SM.
 template <int kGroup>
 __device__ __forceinline__ void TmemAlloc(uint32_t smem_dst, uint32_t columns) {
