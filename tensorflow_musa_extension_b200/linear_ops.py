@@ -107,7 +107,7 @@ def MusaMatMulBiasAct(a, b, bias=None, residual=None, activation="Identity", tra
     transpose_b), bias [n], residual of y's shape [..., n]; bias and residual may be
     None.  activation: "Identity", "Relu", "Sigmoid", "Silu" (z * sigmoid(z); not
     MusaBiasAddSwish, whose factor is the input before the bias) or "Gelu" (z *
-    Phi(z)).  The product and what follows are fp32, y is rounded once.  With
+    Phi(z), good to 1.5e-7 of |z|).  The product and what follows are fp32, y is rounded once.  With
     return_preactivation returns (y, preactivation): z = op(a) op(b) + bias rounded
     to T, which MusaMatMulBiasActGrad takes.  The order of the sums is fixed by the
     sizes; float is not taken: the tensor cores would keep 11 of its 24 bits."""
