@@ -229,12 +229,14 @@ def MusaQuantizedMatMulBiasAct(a, a_scale, b, b_scale, bias=None, residual=None,
             fa, lda = a2.contiguous(), k
         if tb:
             fb, ldb = b.contiguous(), k
+        # Copies are held until the launch: the block of one that is gone is the next one's.
+        sa, sb = a_scale.contiguous(), b_scale.contiguous()
         ws = _r._scratch(lib.MatMulWorkspaceBytes(1, _r._ptr(fa), lda, False, _r._ptr(fb), ldb,
                                                   True, m, n, k), a.device)
         rc = lib.LaunchQuantizedMatMulBiasAct(
-            _r._DT_CODE[out_dtype], _r._ptr(fa), lda, _r._ptr(a_scale.contiguous()), _r._ptr(fb),
-            ldb, _r._ptr(b_scale.contiguous()), _r._ptr(bias), _r._ptr(residual), _r._ptr(y), m,
-            n, k, act, _r._ptr(ws), ws.numel(), _r._stream())
+            _r._DT_CODE[out_dtype], _r._ptr(fa), lda, _r._ptr(sa), _r._ptr(fb), ldb, _r._ptr(sb),
+            _r._ptr(bias), _r._ptr(residual), _r._ptr(y), m, n, k, act, _r._ptr(ws), ws.numel(),
+            _r._stream())
         _r._check(rc, what)
     return y
 

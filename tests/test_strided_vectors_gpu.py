@@ -1,0 +1,52 @@
+"""Vector arguments that are not contiguous, several of them in one call: the bits of the
+call with contiguous copies, and the formulas in 64 bits.  The tolerances are those of
+test_linear_gpu.py."""
+import pytest
+import torch
+
+import test_linear_gpu as linear
+from tensorflow_musa_extension_b200 import raw_ops
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+_rand, _check = linear._rand, linear._check
+
+
+def _every_second(t):
+    return torch.stack((t, torch.full_like(t, 3.0)), -1).flatten(-2)[..., ::2]
+
+
+def _column(t):
+    """t as a column of a table."""
+    flat = t.reshape(-1)
+    return torch.stack((torch.full_like(flat, 5.0), flat, flat + 1), 1)[:, 1].view(t.shape)
+
+
+STORED = [_every_second, _column]
+
+
+@pytest.mark.parametrize("stored", STORED)
+@pytest.mark.parametrize("m,n,k", [(64, 64, 64), (1, 128, 96), (130, 100, 48), (300, 300, 272)])
+def test_scales_of_8bit_products(kernel_lib, stored, m, n, k):
+    a, sa = linear._quantized(m, k, 1)
+    b, sb = linear._quantized(n, k, 2, k ** -0.5)
+    want, _, tol, _ = linear._forward(a.double() * sa, (b.double() * sb).mT, None, None, "Silu",
+                                      False, False, BF16)
+    plain = raw_ops.MusaQuantizedMatMulBiasAct(a, sa, b, sb, activation="Silu")
+    y = raw_ops.MusaQuantizedMatMulBiasAct(a, stored(sa), b, stored(sb), activation="Silu")
+    _check(y, want, tol, "strided scales")
+    assert torch.equal(y, plain)
+
+
+def test_one_scale_for_all_rows(kernel_lib):
+    m, n, k = 64, 64, 128
+    a, b = (linear._quantized(s, k, i).q for i, s in enumerate((m, n)))
+    sa, sb = torch.full((1, 1), 0.25, device="cuda"), torch.full((1, 1), 8.0, device="cuda")
+    want, _, tol, _ = linear._forward(a.double() * 0.25, (b.double() * 8.0).mT, None, None,
+                                      "Identity", False, False, F16)
+    y = raw_ops.MusaQuantizedMatMulBiasAct(a, sa.expand(m, 1), b, sb.expand(n, 1), out_dtype=F16)
+    # Half ends at 65504; what rounds to 65520 and more is infinite.
+    inside, beyond = want.abs() + tol < 65504, want.abs() - tol >= 65520
+    assert inside.any() and torch.equal(y[beyond].double(), want[beyond].sign() * float("inf"))
+    _check(y[inside], want[inside], tol[inside], "expanded scales")
