@@ -216,13 +216,13 @@ def MusaAddRmsNorm(x, residual, gamma, epsilon=0.00001, name=None):
     hf = _r._HostForm()
     xd, rd, g = (hf.to_device(t) for t in (x, residual, gamma))
     rows, last = _check_rows("MusaAddRmsNorm", xd, [("residual", rd, False), ("gamma", g, True)])
-    xd, rd = xd.contiguous(), rd.contiguous()
+    xd, rd, g = xd.contiguous(), rd.contiguous(), g.contiguous()
     with torch.cuda.device(xd.device):
         y, total = torch.empty_like(xd), torch.empty_like(xd)
         inv = torch.empty(tuple(xd.shape[:-1]) + (1,), dtype=torch.float32, device=xd.device)
         fn = getattr(_r._lib(), "LaunchAddRmsNorm_" + _r._SUFFIX[xd.dtype])
-        rc = fn(_r._ptr(xd), _r._ptr(rd), _r._ptr(g.contiguous()), _r._ptr(y), _r._ptr(total),
-                _r._ptr(inv), rows, last, float(epsilon), _r._stream())
+        rc = fn(_r._ptr(xd), _r._ptr(rd), _r._ptr(g), _r._ptr(y), _r._ptr(total), _r._ptr(inv),
+                rows, last, float(epsilon), _r._stream())
         _r._check(rc, "MusaAddRmsNorm")
     return MusaAddRmsNormOutput(*hf.back_many([y, total, inv]))
 
@@ -243,7 +243,8 @@ def MusaAddRmsNormGrad(dy, dsum, sum, inv_rms, gamma, name=None):
     if inv.dtype != torch.float32 or inv.numel() != rows or inv.device != s.device:
         raise InvalidArgumentError(
             "MusaAddRmsNormGrad: inv_rms must be float32 with one value per row (%d)" % rows)
-    s, d = s.contiguous(), d.contiguous()
+    # Copies are held until the launch: the block of one that is gone is the next one's.
+    s, d, inv, g = (t.contiguous() for t in (s, d, inv, g))
     ds = None if ds is None else ds.contiguous()
     with torch.cuda.device(s.device):
         dx, dgamma = torch.empty_like(s), torch.empty_like(g)
@@ -251,9 +252,8 @@ def MusaAddRmsNormGrad(dy, dsum, sum, inv_rms, gamma, name=None):
             lib = _r._lib()
             ws = _r._scratch(lib.AddRmsNormGradWorkspaceBytes(rows, last), s.device)
             fn = getattr(lib, "LaunchAddRmsNormGrad_" + _r._SUFFIX[s.dtype])
-            rc = fn(_r._ptr(d), _r._ptr(ds), _r._ptr(s), _r._ptr(inv.contiguous()),
-                    _r._ptr(g.contiguous()), _r._ptr(dx), _r._ptr(dgamma), rows, last,
-                    _r._ptr(ws), ws.numel(), _r._stream())
+            rc = fn(_r._ptr(d), _r._ptr(ds), _r._ptr(s), _r._ptr(inv), _r._ptr(g), _r._ptr(dx),
+                    _r._ptr(dgamma), rows, last, _r._ptr(ws), ws.numel(), _r._stream())
             _r._check(rc, "MusaAddRmsNormGrad")
     return MusaAddRmsNormGradOutput(*hf.back_many([dx, dgamma]))
 
@@ -270,15 +270,14 @@ def _quantize(opname, x, residual, gamma, epsilon):
             "%s: 8-bit outputs have no host form: pass device tensors" % opname)
     rows, last = _check_rows(opname, xd, [("residual", rd, False), ("gamma", g, True)])
     xd = xd.contiguous()
-    rd = None if rd is None else rd.contiguous()
+    rd, g = (None if t is None else t.contiguous() for t in (rd, g))
     with torch.cuda.device(xd.device):
         q = torch.empty(xd.shape, dtype=torch.float8_e4m3fn, device=xd.device)
         scale = torch.empty(tuple(xd.shape[:-1]) + (1,), dtype=torch.float32, device=xd.device)
         total = None if rd is None else torch.empty_like(xd)
         fn = getattr(_r._lib(), "LaunchAddRmsNormQuantize_" + _r._SUFFIX[xd.dtype])
-        rc = fn(_r._ptr(xd), _r._ptr(rd), _r._ptr(None if g is None else g.contiguous()),
-                _r._ptr(q), _r._ptr(scale), _r._ptr(total), rows, last, float(epsilon),
-                _r._stream())
+        rc = fn(_r._ptr(xd), _r._ptr(rd), _r._ptr(g), _r._ptr(q), _r._ptr(scale),
+                _r._ptr(total), rows, last, float(epsilon), _r._stream())
         _r._check(rc, opname)
     return q, scale, total
 

@@ -50,3 +50,19 @@ def test_one_scale_for_all_rows(kernel_lib):
     inside, beyond = want.abs() + tol < 65504, want.abs() - tol >= 65520
     assert inside.any() and torch.equal(y[beyond].double(), want[beyond].sign() * float("inf"))
     _check(y[inside], want[inside], tol[inside], "expanded scales")
+
+
+@pytest.mark.parametrize("stored", STORED)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,cols", [(64, 64), (100, 100), (300, 512)])
+def test_vectors_of_the_residual_norm(kernel_lib, stored, dtype, rows, cols):
+    x, r, dy = (_rand((rows, cols), dtype, i) for i in (1, 2, 3))
+    g = _rand((cols,), dtype, 4)
+    f = raw_ops.MusaAddRmsNorm(x, r, g)
+    want = (*f, *raw_ops.MusaAddRmsNormGrad(dy, r, f.sum, f.inv_rms, g),
+            *raw_ops.MusaAddRmsNormQuantize(x, r, g))
+    got = (*raw_ops.MusaAddRmsNorm(x, r, stored(g)),
+           *raw_ops.MusaAddRmsNormGrad(dy, r, f.sum, stored(f.inv_rms), stored(g)),
+           *raw_ops.MusaAddRmsNormQuantize(x, r, stored(g)))
+    for a, b in zip(got, want):
+        assert a.shape == b.shape and torch.equal(a.view(torch.uint8), b.view(torch.uint8))
