@@ -58,13 +58,14 @@ def MusaLayerNorm(x, gamma, beta, epsilon=0.00001, name=None):
     rows, last = _rows(xd)
     _check_vector(g, "Gamma", last)
     _check_vector(b, "Beta", last)
-    xd = xd.contiguous()
+    # Copies are held until the launch: the block of one that is gone is the next one's.
+    xd, g, b = xd.contiguous(), g.contiguous(), b.contiguous()
     with torch.cuda.device(xd.device):
         y = torch.empty_like(xd)
         if xd.numel():
             fn = getattr(_r._lib(), "LaunchLayerNorm_" + _r._SUFFIX[xd.dtype])
-            rc = fn(_r._ptr(xd), _r._ptr(g.contiguous()), _r._ptr(b.contiguous()), _r._ptr(y),
-                    None, None, rows, last, float(epsilon), _r._stream())
+            rc = fn(_r._ptr(xd), _r._ptr(g), _r._ptr(b), _r._ptr(y), None, None, rows, last,
+                    float(epsilon), _r._stream())
             _r._check(rc, "MusaLayerNorm")
     return hf.back(y)
 
@@ -93,7 +94,7 @@ def MusaLayerNormGrad(dy, x, gamma, beta, epsilon=0.00001, name=None):
     rows, last = _rows(xd)
     _check_vector(g, "Gamma", last)
     _check_vector(b, "Beta", last)
-    xd, d = xd.contiguous(), d.contiguous()
+    xd, d, g = xd.contiguous(), d.contiguous(), g.contiguous()
     with torch.cuda.device(xd.device):
         dx = torch.empty_like(xd)
         dgamma = torch.empty_like(g)
@@ -103,9 +104,9 @@ def MusaLayerNormGrad(dy, x, gamma, beta, epsilon=0.00001, name=None):
             nbytes = lib.LayerNormGradWorkspaceBytes(rows, last)
             ws = _r._workspace(nbytes, xd.device)
             fn = getattr(lib, "LaunchLayerNormGrad_" + _r._SUFFIX[xd.dtype])
-            rc = fn(_r._ptr(d), _r._ptr(xd), _r._ptr(g.contiguous()), _r._ptr(dx),
-                    _r._ptr(dgamma), _r._ptr(dbeta), rows, last, float(epsilon), _r._ptr(ws),
-                    ws.numel(), _r._stream())
+            rc = fn(_r._ptr(d), _r._ptr(xd), _r._ptr(g), _r._ptr(dx), _r._ptr(dgamma),
+                    _r._ptr(dbeta), rows, last, float(epsilon), _r._ptr(ws), ws.numel(),
+                    _r._stream())
             _r._check(rc, "MusaLayerNormGrad")
     return MusaLayerNormGradOutput(*hf.back_many([dx, dgamma, dbeta]))
 
@@ -129,7 +130,7 @@ def MusaRmsNorm(x, gamma, epsilon=0.00001, name=None):
         raise InvalidArgumentError("Last dimension must be positive")
     _check_vector(g, "Gamma", last)
     rows = xd.numel() // last
-    xd = xd.contiguous()
+    xd, g = xd.contiguous(), g.contiguous()
     with torch.cuda.device(xd.device):
         y = torch.empty_like(xd)
         normalized = torch.empty_like(xd)
@@ -137,8 +138,8 @@ def MusaRmsNorm(x, gamma, epsilon=0.00001, name=None):
         if xd.numel():
             lib = _r._lib()
             fn = lib.LaunchRmsNormFloat if xd.dtype == torch.float32 else lib.LaunchRmsNormBFloat16
-            fn(_r._ptr(xd), _r._ptr(g.contiguous()), _r._ptr(y), _r._ptr(normalized),
-               _r._ptr(inv), rows, last, float(epsilon), _r._stream())
+            fn(_r._ptr(xd), _r._ptr(g), _r._ptr(y), _r._ptr(normalized), _r._ptr(inv), rows,
+               last, float(epsilon), _r._stream())
     return MusaRmsNormOutput(*hf.back_many([y, normalized, inv]))
 
 
@@ -163,15 +164,15 @@ def MusaRmsNormGradDx(x, inv_rms, gamma, dy, name=None):
     rows = xd.numel() // last
     if inv.numel() != rows:
         raise InvalidArgumentError("MusaRmsNormGradDx inv size mismatch")
-    xd, d = xd.contiguous(), d.contiguous()
+    xd, inv, g, d = (t.contiguous() for t in (xd, inv, g, d))
     with torch.cuda.device(xd.device):
         dx = torch.empty_like(xd)
         if xd.numel():
             lib = _r._lib()
             fn = (lib.LaunchRmsNormGradDxFloat if xd.dtype == torch.float32
                   else lib.LaunchRmsNormGradDxBFloat16)
-            fn(_r._ptr(xd), _r._ptr(inv.contiguous()), _r._ptr(g.contiguous()), _r._ptr(d),
-               _r._ptr(dx), rows, last, _r._stream())
+            fn(_r._ptr(xd), _r._ptr(inv), _r._ptr(g), _r._ptr(d), _r._ptr(dx), rows, last,
+               _r._stream())
     return hf.back(dx)
 
 

@@ -66,3 +66,18 @@ def test_vectors_of_the_residual_norm(kernel_lib, stored, dtype, rows, cols):
            *raw_ops.MusaAddRmsNormQuantize(x, r, stored(g)))
     for a, b in zip(got, want):
         assert a.shape == b.shape and torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("stored", STORED)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,cols", [(64, 64), (100, 100), (300, 512)])
+def test_vectors_of_the_row_norms(kernel_lib, stored, dtype, rows, cols):
+    x, dy = (_rand((rows, cols), dtype, i) for i in (1, 2))
+    g, b = _rand((cols,), dtype, 3), _rand((cols,), dtype, 4)
+    inv = raw_ops.MusaRmsNorm(x, g).inv_rms
+
+    def all_of(g, b, inv):
+        return (raw_ops.MusaLayerNorm(x, g, b), *raw_ops.MusaLayerNormGrad(dy, x, g, b),
+                *raw_ops.MusaRmsNorm(x, g), raw_ops.MusaRmsNormGradDx(x, inv, g, dy))
+    for got, want in zip(all_of(stored(g), stored(b), stored(inv)), all_of(g, b, inv)):
+        assert got.shape == want.shape and torch.equal(got, want)
