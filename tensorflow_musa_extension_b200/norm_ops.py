@@ -98,7 +98,7 @@ def MusaLayerNormGrad(dy, x, gamma, beta, epsilon=0.00001, name=None):
     with torch.cuda.device(xd.device):
         dx = torch.empty_like(xd)
         dgamma = torch.empty_like(g)
-        dbeta = torch.empty_like(b)
+        dbeta = torch.empty_like(b, memory_format=torch.contiguous_format)
         if last:
             lib = _r._lib()
             nbytes = lib.LayerNormGradWorkspaceBytes(rows, last)

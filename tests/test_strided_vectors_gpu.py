@@ -81,3 +81,18 @@ def test_vectors_of_the_row_norms(kernel_lib, stored, dtype, rows, cols):
                 *raw_ops.MusaRmsNorm(x, g), raw_ops.MusaRmsNormGradDx(x, inv, g, dy))
     for got, want in zip(all_of(stored(g), stored(b), stored(inv)), all_of(g, b, inv)):
         assert got.shape == want.shape and torch.equal(got, want)
+
+
+def test_gradients_of_vectors_with_two_axes(kernel_lib):
+    """Vectors are taken by their number of values; one of two axes, stored with the first
+    contiguous, has its gradients in the order of its values."""
+    x, dy = _rand((70, 24), F32, 1), _rand((70, 24), F32, 2)
+    g, b = _rand((24,), F32, 3), _rand((24,), F32, 4)
+    inv = raw_ops.MusaRmsNorm(x, g).inv_rms
+
+    def both(g, b):
+        return (*raw_ops.MusaLayerNormGrad(dy, x, g, b)[1:],
+                raw_ops.MusaAddRmsNormGrad(dy, None, x, inv, g).dgamma)
+    tables = (t.view(4, 6).t().contiguous().t() for t in (g, b))
+    for got, want in zip(both(*tables), both(g, b)):
+        assert got.shape == (4, 6) and torch.equal(got.reshape(-1), want)
