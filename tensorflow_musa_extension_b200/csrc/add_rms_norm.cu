@@ -230,8 +230,9 @@ __global__ void __launch_bounds__(1024) AddNormKernel(AddNormArgs a) {
   const T* next_x = static_cast<const T*>(a.x) + view.first + t * kVec;
   const T* next_r = add ? static_cast<const T*>(a.residual) + view.first + t * kVec : nullptr;
   int64_t next_row = row;
-  // The tensor's last pack: what lies behind it is not read and comes as zeros.
-  const int tail = view.row_size + view.shift - (view.packs - 1) * kVec;
+  // What lies behind the tensor is not read and comes as zeros (rows shorter than a pack share
+  // the last one).
+  const int64_t first_tail_row = FirstTailRow<kVec>(a.rows, a.row_size);
   // One group of copies, maybe empty.
   const auto Ask = [&](char* stage) {
     if (next_row < a.rows) {
@@ -241,9 +242,12 @@ __global__ void __launch_bounds__(1024) AddNormKernel(AddNormArgs a) {
         if (p < view.packs) {
           uint4* x_slot = reinterpret_cast<uint4*>(stage + j * pitch);
           uint4* r_slot = reinterpret_cast<uint4*>(stage + (kPacks + j) * pitch);
-          if (kShifted && next_row == a.rows - 1 && p == view.packs - 1) {
-            CopyPart(x_slot, next_x + j * hop, tail * static_cast<int>(sizeof(T)));
-            if (add) CopyPart(r_slot, next_r + j * hop, tail * static_cast<int>(sizeof(T)));
+          const int inside = kShifted ? ElementsInside<kVec>(next_row, a.rows, first_tail_row,
+                                                             a.row_size, view.shift, p, view.packs)
+                                      : kVec;
+          if (inside < kVec) {
+            CopyPart(x_slot, next_x + j * hop, inside * static_cast<int>(sizeof(T)));
+            if (add) CopyPart(r_slot, next_r + j * hop, inside * static_cast<int>(sizeof(T)));
           } else {
             CopyPack(x_slot, next_x + j * hop);
             if (add) CopyPack(r_slot, next_r + j * hop);

@@ -49,4 +49,19 @@ MUSA_HOST_DEVICE constexpr int PackElements(int64_t row, int64_t rows, int row_s
   return left < kVec ? left : kVec;
 }
 
+// The first row whose last pack can be the tensor's, whatever the length of the rows.
+template <int kVec>
+MUSA_HOST_DEVICE constexpr int64_t FirstTailRow(int64_t rows, int row_size) {
+  return rows - (row_size < kVec ? kVec : 1);
+}
+
+// Elements of the row's pack p (of `packs`) that lie inside the tensor.
+template <int kVec>
+MUSA_HOST_DEVICE constexpr int ElementsInside(int64_t row, int64_t rows, int64_t first_tail_row,
+                                              int row_size, int shift, int p, int packs) {
+  return p == packs - 1 && row >= first_tail_row
+             ? PackElements<kVec, kVec>(row, rows, row_size, shift, p)
+             : kVec;
+}
+
 }  // namespace musa_b200
