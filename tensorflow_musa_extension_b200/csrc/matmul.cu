@@ -1335,7 +1335,9 @@ extern "C" {
 
 int MusaMatMulStatus(void) {
   int v = 0;
-  const cudaError_t rc = cudaMemcpyFromSymbol(&v, g_status, sizeof(v));
+  // The copy alone would not wait for streams that do not block with the default one.
+  cudaError_t rc = cudaDeviceSynchronize();
+  if (rc == cudaSuccess) rc = cudaMemcpyFromSymbol(&v, g_status, sizeof(v));
   return rc != cudaSuccess ? static_cast<int>(rc) : v == 0 ? MUSA_KERNELS_OK : MUSA_KERNELS_EGAVEUP;
 }
 
