@@ -1069,6 +1069,9 @@ Plan PlanProduct(int64_t m, int64_t n, int blocks, bool a_rows) {
   if (form >= 16) {
     best.rows_tile = Tile(form & ~15);
     best.splits = form & 15;
+    // Every CTA of a cluster multiplies: one without a block of depth would hand on what its
+    // tensor memory held before.
+    while (best.splits > 1 && best.splits > blocks) best.splits /= 2;
   } else if (blocks > 0 && (form == 2 || form == 3)) {
     best.tile_n = form == 2 ? 256 : 128;
   } else if (blocks > 0) {
