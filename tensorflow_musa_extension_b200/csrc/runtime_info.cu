@@ -28,6 +28,14 @@ void InitTuningOnce() {
     for (int i = 0; i < kTuneCount; ++i) g_tuning[i].store(defaults[i]);
   });
 }
+
+// Row tiles of whole instructions, and cluster sizes that divide them.
+bool KnownMatMulForm(int value) {
+  const int rows = value & ~15, splits = value & 15;
+  return (value >= 0 && value <= 3) ||
+         (rows >= 16 && rows <= 256 &&
+          (splits == 1 || splits == 2 || splits == 4 || splits == 8));
+}
 }  // namespace
 
 int SmCount() {
@@ -63,10 +71,12 @@ const char* MusaKernelsVersion(void) {
 int MusaKernelsTargetArch(void) { return 100; }
 
 // Sweep/test hook, not part of the reference boundary: sets one launch-shape
-// knob for the whole process and returns the previous value (-1: bad key).
+// knob for the whole process and returns the previous value (-1: bad key, or a form of
+// the matrix products that there is not).
 int MusaKernelsSetTuning(int key, int value) {
   musa_b200::InitTuningOnce();
   if (key < 0 || key >= musa_b200::kTuneCount) return -1;
+  if (key == musa_b200::kTuneMatMulForm && !musa_b200::KnownMatMulForm(value)) return -1;
   return musa_b200::g_tuning[key].exchange(value);
 }
 
