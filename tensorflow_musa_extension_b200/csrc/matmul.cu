@@ -208,7 +208,8 @@ __device__ __forceinline__ void FinishColumn(float (&v)[kN], const ColumnInputs<
   T* y = static_cast<T*>(e.y) + row * a.n + col;
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
-    if constexpr (kBytes) v[i] *= in.scale[i] * col_scale;
+    // One scale after the other: the product of the two may leave fp32's range.
+    if constexpr (kBytes) v[i] = v[i] * in.scale[i] * col_scale;
     v[i] += bias;
   }
   if (e.z != nullptr) {
@@ -694,10 +695,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           WidenPack<4>(*reinterpret_cast<const Pack<T, 4>*>(&bias_of[group][c + i]), b);
           if constexpr (kBytes) {
             const float4 w = *reinterpret_cast<const float4*>(&scale_of[group][c + i]);
-            v[i] *= row_scale * w.x;
-            v[i + 1] *= row_scale * w.y;
-            v[i + 2] *= row_scale * w.z;
-            v[i + 3] *= row_scale * w.w;
+            v[i] = v[i] * row_scale * w.x;
+            v[i + 1] = v[i + 1] * row_scale * w.y;
+            v[i + 2] = v[i + 2] * row_scale * w.z;
+            v[i + 3] = v[i + 3] * row_scale * w.w;
           }
           v[i] += b[0].x;
           v[i + 1] += b[0].y;
