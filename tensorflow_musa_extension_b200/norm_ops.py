@@ -15,6 +15,7 @@ from . import raw_ops as _r
 
 _LN_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 _RMS_DTYPES = (torch.float32, torch.bfloat16)
+_SCALE_MIN = 2.0 ** -126
 
 MusaLayerNormGradOutput = collections.namedtuple(
     "MusaLayerNormGrad", ["dx", "dgamma", "dbeta"])
@@ -178,13 +179,16 @@ def MusaRmsNormGradDx(x, inv_rms, gamma, dy, name=None):
 
 # ------------------------------------------ RMS norm of a residual's sum --
 
-def _check_rows(opname, x, others):
-    """x's rows and their length; `others`: (name, tensor, like x or a vector)."""
+def _check_rows(opname, x, others, normed=True):
+    """x's rows and their length; `others`: (name, tensor, like x or a vector).  Rows of length
+    0 have no norm."""
     if x.dtype not in _LN_DTYPES:
         raise InvalidArgumentError("%s: unsupported dtype %s" % (opname, x.dtype))
     if x.dim() < 1:
         raise InvalidArgumentError("Input rank must be >= 1")
     rows, last = _rows(x)
+    if normed and not last:
+        raise InvalidArgumentError("%s: the last dimension must be positive" % opname)
     for name, t, vector in others:
         if t is None:
             continue
@@ -209,7 +213,8 @@ def MusaAddRmsNorm(x, residual, gamma, epsilon=0.00001, name=None):
     residual, inv_rms = rsqrt(mean(sum^2) + epsilon) (fp32, shaped like x with a
     last axis of 1) and y = sum * inv_rms * gamma.  The norm is that of the
     unrounded sum; `sum` holds it rounded to T.  One launch where Add and
-    MusaRmsNorm are two with the sum written and read between."""
+    MusaRmsNorm are two with the sum written and read between.  Rows of length 0
+    have no norm and are refused."""
     out = _r._native().add_rms_norm(x, residual, gamma, epsilon)
     if out is not None:
         return _r._native_result(out, MusaAddRmsNormOutput, "MusaAddRmsNorm")
@@ -249,13 +254,12 @@ def MusaAddRmsNormGrad(dy, dsum, sum, inv_rms, gamma, name=None):
     ds = None if ds is None else ds.contiguous()
     with torch.cuda.device(s.device):
         dx, dgamma = torch.empty_like(s), torch.empty_like(g)
-        if last:
-            lib = _r._lib()
-            ws = _r._scratch(lib.AddRmsNormGradWorkspaceBytes(rows, last), s.device)
-            fn = getattr(lib, "LaunchAddRmsNormGrad_" + _r._SUFFIX[s.dtype])
-            rc = fn(_r._ptr(d), _r._ptr(ds), _r._ptr(s), _r._ptr(inv), _r._ptr(g), _r._ptr(dx),
-                    _r._ptr(dgamma), rows, last, _r._ptr(ws), ws.numel(), _r._stream())
-            _r._check(rc, "MusaAddRmsNormGrad")
+        lib = _r._lib()
+        ws = _r._scratch(lib.AddRmsNormGradWorkspaceBytes(rows, last), s.device)
+        fn = getattr(lib, "LaunchAddRmsNormGrad_" + _r._SUFFIX[s.dtype])
+        rc = fn(_r._ptr(d), _r._ptr(ds), _r._ptr(s), _r._ptr(inv), _r._ptr(g), _r._ptr(dx),
+                _r._ptr(dgamma), rows, last, _r._ptr(ws), ws.numel(), _r._stream())
+        _r._check(rc, "MusaAddRmsNormGrad")
     return MusaAddRmsNormGradOutput(*hf.back_many([dx, dgamma]))
 
 
@@ -269,12 +273,15 @@ def _quantize(opname, x, residual, gamma, epsilon):
     if hf.kind is not None:
         raise InvalidArgumentError(
             "%s: 8-bit outputs have no host form: pass device tensors" % opname)
-    rows, last = _check_rows(opname, xd, [("residual", rd, False), ("gamma", g, True)])
+    rows, last = _check_rows(opname, xd, [("residual", rd, False), ("gamma", g, True)],
+                             normed=g is not None)
     xd = xd.contiguous()
     rd, g = (None if t is None else t.contiguous() for t in (rd, g))
     with torch.cuda.device(xd.device):
         q = torch.empty(xd.shape, dtype=torch.float8_e4m3fn, device=xd.device)
         scale = torch.empty(tuple(xd.shape[:-1]) + (1,), dtype=torch.float32, device=xd.device)
+        if not last:                 # nothing is launched: the least scale, as for a row of zeros
+            scale.fill_(_SCALE_MIN)
         total = None if rd is None else torch.empty_like(xd)
         fn = getattr(_r._lib(), "LaunchAddRmsNormQuantize_" + _r._SUFFIX[xd.dtype])
         rc = fn(_r._ptr(xd), _r._ptr(rd), _r._ptr(g), _r._ptr(q), _r._ptr(scale),
@@ -288,7 +295,7 @@ def MusaAddRmsNormQuantize(x, residual, gamma, epsilon=0.00001, name=None):
     float8_e4m3fn and scale = max(max|y| / 448, 2^-126) of each row (fp32, shaped
     like x with a last axis of 1), so that y = q * scale; y itself is not written.
     `residual` None: the norm of x alone, and sum is None.  A row with a NaN has a
-    NaN scale; rows of length 0 have none."""
+    NaN scale; rows of length 0 have no norm and are refused."""
     if gamma is None:
         raise InvalidArgumentError("MusaAddRmsNormQuantize: gamma is missing")
     out = _quantize("MusaAddRmsNormQuantize", x, residual, gamma, epsilon)
@@ -298,5 +305,6 @@ def MusaAddRmsNormQuantize(x, residual, gamma, epsilon=0.00001, name=None):
 def MusaQuantizeRows(x, name=None):
     """The rows of x (T in {float, half, bfloat16}) in 8 bits: returns (q, scale),
     x = q * scale, as MusaAddRmsNormQuantize returns them; what lays out the weights
-    [n, k] of MusaQuantizedMatMulBiasAct once."""
+    [n, k] of MusaQuantizedMatMulBiasAct once.  A row of length 0 has the least scale,
+    2^-126, as a row of zeros has."""
     return MusaQuantizeRowsOutput(*_quantize("MusaQuantizeRows", x, None, None, 0.0)[:2])
