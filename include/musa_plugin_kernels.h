@@ -481,9 +481,10 @@ int LaunchAddRmsNormGrad_BF16(const void* dy, const void* dsum, const void* sum,
                               size_t workspace_bytes, cudaStream_t stream);
 
 /* The same forward with its output in 8 bits: scale[row] = max(max|y| / 448, 2^-126), fp32;
- * q = e4m3(y / scale), rounded to nearest even.  y is not written.  `residual` and `sum` may
+ * q = e4m3(y / scale), rounded to nearest even (behind a norm the quotient is good to a few
+ * fp32 roundings, as y is; rows as they are take one rounded division).  y is not written.  `residual` and `sum` may
  * both be null (the norm of x alone); with `gamma` null too the rows of x are quantised as
- * they are.  A NaN in a row makes its scale NaN. */
+ * they are.  A NaN in a row makes its scale NaN.  Nothing is written where row_size is 0. */
 int LaunchAddRmsNormQuantize_F32(const void* x, const void* residual, const void* gamma,
                                  void* q, float* scale, void* sum, int64_t rows,
                                  int64_t row_size, float epsilon, cudaStream_t stream);
@@ -532,7 +533,7 @@ int LaunchMatMulBiasActGrad(int dtype, const void* dy, const void* a, int64_t ld
                             size_t workspace_bytes, cudaStream_t stream);
 
 /* The product of e4m3 factors with fp32 scales: z = (a b^T) * a_scale[row] * b_scale[column]
- * + bias; y = act(z) + residual.  a: lines of k bytes, `lda` apart, [m, k]; b: [n, k].  bias,
+ * + bias, in this order; y = act(z) + residual.  a: lines of k bytes, `lda` apart, [m, k]; b: [n, k].  bias,
  * residual and y are of out_dtype (MUSA_DT_F16 or MUSA_DT_BF16). */
 int LaunchQuantizedMatMulBiasAct(int out_dtype, const void* a, int64_t lda,
                                  const float* a_scale, const void* b, int64_t ldb,
@@ -946,9 +947,11 @@ long long MusaKernelsLaunchCount(void);
 /* Test and sweep hooks, not part of the reference boundary: launch-shape
  * knobs (grid sizes, pipeline depths, cache hints; csrc/tuning.h lists the
  * keys) that let a sweep compare variants without rebuilding.  They change
- * HOW a launcher runs, never what it computes.  The table is process-wide and
+ * HOW a launcher runs, never what it computes (the form of the matrix products
+ * changes the order of their sums).  The table is process-wide and
  * is read by every launcher at every call: set a knob only while no other
- * thread is launching.  Set returns the previous value (-1: unknown key). */
+ * thread is launching.  Set returns the previous value (-1: unknown key, or a
+ * form of the matrix products that there is not: nothing is set). */
 int MusaKernelsSetTuning(int key, int value);
 int MusaKernelsGetTuning(int key);
 

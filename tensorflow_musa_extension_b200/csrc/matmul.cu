@@ -52,7 +52,10 @@ __device__ __forceinline__ float2 SigmoidOf(float2 z) {
 
 // Phi(-|z|), and exp(-z^2 / 2) in `*bell`.  Hastings' rational form of the error function
 // (Abramowitz and Stegun 7.1.26): with t = 1 / (1 + p |z| / sqrt 2), erfc(|z| / sqrt 2) is
-// a polynomial of degree five in t times the bell, to 1.5e-7.  erff, which takes a branch at
+// a polynomial of degree five in t times the bell, to 1.5e-7 (the polynomial alone; with the
+// roundings of fp32 and the two hardware functions z Phi(z) is off by up to 8e-7 of |z|).  The
+// bound is absolute: where the value itself is small, below z = -5, it is good to 0.4 % down to
+// -6 and to 1 % down to -8 (an fp32 1 + erf has lost it all there).  erff, which takes a branch at
 // 1 and some 40 instructions, made the epilogue of a tile three times as long (8192 x 16384
 // outputs of depth 64: 225 us against 108 without an activation).
 __device__ __forceinline__ float2 NormalTail(float2 z, float2* bell) {
@@ -1022,8 +1025,11 @@ struct Plan {
 // taken from a sweep of every form over 160 sizes (1 .. 2000 rows, both factor types): the
 // longest of the depth steps of the waves of CTAs one after the other, the factors' copies
 // out of L2 and the reads of HBM; then the epilogues of the waves, which a split tile pays with
-// the exchange of its partial sums.  Over that sweep the choice was 5% off the best form in
-// the mean; fixed tiles of 256 rows were 35% off (1000 x 640, depth 1408: 19.2 us against 8.9;
+// the exchange of its partial sums.  Over that sweep the choice was 4% off the best form in
+// the mean and 1.79 times at the worst (100 x 640, depth 1408: 12.3 us against 6.8; then
+// 64 x 16384, depth 256: 8.2 against 6.2).  It holds sizes whose lines are whole 16 bytes; the
+// other sizes go by the same rule, which does not know what their outputs cost the split form
+// (16 sizes with all outputs, half of them odd: 6% and 1.27).  Fixed tiles of 256 rows were 35% off (1000 x 640, depth 1408: 19.2 us against 8.9;
 // 256 x 1000, depth 520: 15.7 against 6.6; one row x 4096, depth 4096: 12.1 against 11.0).
 constexpr double kMbPerUs = 1e-6;
 

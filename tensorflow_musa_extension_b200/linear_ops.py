@@ -107,8 +107,9 @@ def MusaMatMulBiasAct(a, b, bias=None, residual=None, activation="Identity", tra
     transpose_b), bias [n], residual of y's shape [..., n]; bias and residual may be
     None.  activation: "Identity", "Relu", "Sigmoid", "Silu" (z * sigmoid(z); not
     MusaBiasAddSwish, whose factor is the input before the bias) or "Gelu" (z *
-    Phi(z), good to 1.5e-7 of |z|).  The product and what follows are fp32, y is rounded once.  With
-    return_preactivation returns (y, preactivation): z = op(a) op(b) + bias rounded
+    Phi(z), good to 8e-7 of |z|; of the value, which is small there, to 0.4 % at
+    z = -6 and 1 % at -8).  The product and what follows are fp32, y is rounded
+    once.  With return_preactivation returns (y, preactivation): z = op(a) op(b) + bias rounded
     to T, which MusaMatMulBiasActGrad takes.  The order of the sums is fixed by the
     sizes; float is not taken: the tensor cores would keep 11 of its 24 bits."""
     what = "MusaMatMulBiasAct"
@@ -196,7 +197,7 @@ def MusaQuantizedMatMulBiasAct(a, a_scale, b, b_scale, bias=None, residual=None,
                                activation="Identity", out_dtype=torch.bfloat16, name=None):
     """y = act((a * a_scale) (b * b_scale)^T + bias) + residual for float8_e4m3fn a
     [..., k] and b [n, k] with fp32 scales, one per row of each (MusaQuantizeRows,
-    MusaAddRmsNormQuantize); bias [n], residual [..., n] and y are of out_dtype,
+    MusaAddRmsNormQuantize), which the product takes one after the other; bias [n], residual [..., n] and y are of out_dtype,
     half or bfloat16.  Device tensors only."""
     what = "MusaQuantizedMatMulBiasAct"
     act = _activation(what, activation)
