@@ -245,7 +245,8 @@ def MusaQuantizedMatMulBiasAct(a, a_scale, b, b_scale, bias=None, residual=None,
 def check_products():
     """Raises InternalError if a product's kernel on the current device has given up a
     wait since the library was loaded (its outputs are then not valid; the kernels'
-    waits end after about two seconds).  Synchronises with the device."""
+    waits end after about two seconds).  Synchronises with the device: not to be called while
+    a stream is captured."""
     rc = _r._lib().MusaMatMulStatus()
     if rc != 0:
         raise InternalError("matrix products: %s" % _r._capi.ERROR_NAMES.get(rc, rc))
