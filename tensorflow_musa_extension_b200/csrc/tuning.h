@@ -43,7 +43,8 @@ enum TuningKey {
                             // (what the caller does then is tested with it)
   kTuneMatMulForm = 29,     // form of the matrix products: 0 by rule, 1 split, 2 and 3 pairs of CTAs with
                             // tiles of 256 and 128 columns, 16 or more the split form with row
-                            // tiles of `value & ~15` rows and `value & 15` CTAs a tile
+                            // tiles of `value & ~15` rows (16 .. 256) and at most `value & 15`
+                            // CTAs a tile (1, 2, 4 or 8); other values are refused
   kTuneCount = 30
 };
 
